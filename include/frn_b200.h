@@ -67,6 +67,8 @@ extern "C" {
 
 /* Device error-word bits (frn_device_error). */
 #define FRN_DEVERR_WAIT_TIMEOUT  0x1u  /* an mbarrier wait ran out            */
+#define FRN_DEVERR_BAD_PAGE      0x2u  /* a page or a length outside the cache */
+#define FRN_DEVERR_BAD_LENGTH    0x4u  /* cu_seqlens outside the given limits */
 
 /* Version of this ABI; bumped on any signature change. */
 int frn_abi_version(void);
@@ -292,6 +294,109 @@ int frn_gqa_decode_attention_noalloc(int dtype, const void* q, const void* k_cac
                                      int64_t num_q_heads, int64_t num_kv_heads,
                                      int64_t head_dim, int64_t context_len, float scale,
                                      void* stream);
+
+/*
+ * Causal grouped-query attention over packed prompts: sequence b is rows
+ * [cu_seqlens[b], cu_seqlens[b + 1]) of q, k, v and out, and for its token i
+ *     out[i, h, :] = sum_{j <= i} softmax_j(scale * q[i, h, :] . k[j, h/G, :]) v[j, h/G, :]
+ * over the tokens j of the same sequence; G = num_q_heads / num_kv_heads.
+ * q [tokens, num_q_heads, head_dim_qk], k [tokens, num_kv_heads, head_dim_qk],
+ * v [tokens, num_kv_heads, head_dim_v], out [tokens, num_q_heads, head_dim_v],
+ * all `dtype` (fp16 / bf16), with unit stride along the head dim and any token
+ * and head strides (elements, multiples of 8); 16-byte aligned.
+ * (head_dim_qk, head_dim_v) is (64, 64), (128, 128) or (192, 128), G at most
+ * 128.  cu_seqlens: batch + 1 non-decreasing int32 on the device; sequences
+ * may be empty; no sequence may be longer than max_seqlen.  A boundary outside
+ * [0, tokens] or a longer sequence is cut to the limit and reported as
+ * FRN_DEVERR_BAD_LENGTH.  Rows of no sequence are left as they are.
+ * Scores, softmax statistics and output sums are fp32; the probabilities are
+ * rounded to `dtype` for the product with v.  What lies in k and v after
+ * position i has no effect on row i, NaN and infinities included.
+ * Replaces the library call that the reference's patched attention makes for
+ * prompts (reference src/patch_llama.py:147-161).
+ */
+int frn_gqa_prompt_attention(int dtype, const void* q, int64_t q_token_stride,
+                             int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                             int64_t v_head_stride, void* out, int64_t out_token_stride,
+                             int64_t out_head_stride, const int32_t* cu_seqlens, int64_t batch,
+                             int64_t tokens, int64_t max_seqlen, int64_t num_q_heads,
+                             int64_t num_kv_heads, int64_t head_dim_qk, int64_t head_dim_v,
+                             float scale, void* stream);
+
+/*
+ * A paged key-value cache: pools of num_pages pages of page_size tokens, and a
+ * page table that says which page holds which part of a sequence.  Token t of
+ * sequence b has its key for head h at
+ *     k + page * k_page_stride + (t % page_size) * k_token_stride + h * k_head_stride,
+ *     page = page_table[b * page_table_stride + t / page_size]
+ * (strides in elements, positive multiples of 16 bytes; unit stride along
+ * head_dim; 16-byte aligned), and v likewise.  Entries of the table beyond a
+ * sequence's length are not read.  Pages may be shared between sequences.
+ */
+typedef struct frn_paged_kv {
+  void* k;
+  void* v;
+  int64_t num_pages, page_size, num_kv_heads, head_dim;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const int32_t* page_table; /* device, [batch][max_pages] */
+  int64_t page_table_stride, max_pages;
+} frn_paged_kv;
+
+/*
+ * Decode-step grouped-query attention over a paged cache: as
+ * frn_gqa_decode_attention, with the keys and values of sequence b being the
+ * seq_lens[b] (int32, device; 0 gives a row of zeros) first tokens of its pages.
+ * q and out [batch, num_q_heads, head_dim] with unit stride along head_dim and
+ * any batch and head strides (elements, multiples of 16 bytes).  fp32 / fp16 /
+ * bf16; head_dim 64 or 128; any page_size; G at most 16.  The lengths are read
+ * on the device, so a captured call serves a growing cache; the work is cut
+ * into equal shares there.  workspace: at least
+ * frn_gqa_paged_decode_workspace_size bytes, contents immaterial, not shared
+ * by calls that may overlap.  A table entry outside [0, num_pages) reads as
+ * zero keys and values, a length outside [0, max_pages * page_size] is cut to
+ * it; both set FRN_DEVERR_BAD_PAGE.
+ * No counterpart in the reference, whose decode kernels take one contiguous
+ * cache (csrc/gqa_attention_kernel.cu:357-470).
+ */
+size_t frn_gqa_paged_decode_workspace_size(int dtype, int64_t batch, int64_t num_q_heads,
+                                           int64_t num_kv_heads, int64_t head_dim,
+                                           int64_t page_size, int64_t max_pages);
+int frn_gqa_paged_decode_attention(int dtype, const void* q, int64_t q_batch_stride,
+                                   int64_t q_head_stride, const frn_paged_kv* cache,
+                                   const int32_t* seq_lens, void* out, int64_t out_batch_stride,
+                                   int64_t out_head_stride, int64_t batch, int64_t num_q_heads,
+                                   float scale, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/*
+ * Writes new tokens into a paged cache: row t of k and v [tokens,
+ * num_kv_heads, head_dim] (strides in elements, multiples of 16 bytes),
+ * belonging to the sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1],
+ * becomes token start_lens[b] + t - cu_seqlens[b] of that sequence.
+ * cu_seqlens NULL: one token for each of the batch sequences.  start_lens and
+ * cu_seqlens are int32 on the device.  Rows of no sequence are skipped; a row
+ * that has no page within the cache is skipped and sets FRN_DEVERR_BAD_PAGE.
+ * The pages must already be in the table; no two sequences may write to the
+ * same slot.  dtype fp32 / fp16 / bf16.
+ */
+int frn_kv_cache_append(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                        const frn_paged_kv* cache, const int32_t* start_lens,
+                        const int32_t* cu_seqlens, int64_t batch, int64_t tokens, void* stream);
+
+/*
+ * Copies pages within each of npools pools (the K and V pools of all layers,
+ * say): page src[i] to page dst[i] for i < npairs, in every pool.  pools, src
+ * and dst are HOST arrays, read before the call returns.  A page is page_bytes
+ * contiguous bytes, pages are page_stride_bytes apart (multiples of 16), pools
+ * 16-byte aligned and distinct.  Sources may repeat; destinations may not, and
+ * no page may be both (the copies are not ordered).
+ */
+int frn_kv_pages_copy(void* const* pools, int64_t npools, int64_t num_pages, int64_t page_bytes,
+                      int64_t page_stride_bytes, const int32_t* src, const int32_t* dst,
+                      int64_t npairs, void* stream);
 
 /*
  * Reads (and optionally clears) the device error word of `device`, which

@@ -152,6 +152,208 @@ void gqa_decode_v3(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v
   gqa_decode_impl(q, k, v, out, scale, "gqa_decode_v3");
 }
 
+// ---- prompts and the paged key-value cache
+
+// `t` [tokens, heads, dim] as the kernels read it: unit stride along dim,
+// other strides multiples of 16 bytes and no smaller than a head, 16-byte
+// aligned; a copy where it is not.
+at::Tensor heads_legal(const at::Tensor& t) {
+  const int64_t es = t.element_size(), d = t.size(2);
+  bool ok = (t.stride(2) == 1 || d == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 2 && ok; ++i)
+    ok = t.size(i) <= 1 || (t.stride(i) >= d && (t.stride(i) * es) % 16 == 0);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+// Stride of dim i, or that of a contiguous layout where the dim has at most
+// one entry and its stride means nothing.
+int64_t stride_or(const at::Tensor& t, int i) {
+  if (t.size(i) > 1) return t.stride(i);
+  int64_t s = 1;
+  for (int j = t.dim() - 1; j > i; --j) s *= std::max<int64_t>(t.size(j), 1);
+  return s;
+}
+
+void check_ints(const at::Tensor& t, const at::Tensor& on, int dim, const char* name,
+                const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dim && t.device() == on.device(), name,
+              ": ", what, " must be a ", dim, "-D int32 tensor on ", on.device());
+  TORCH_CHECK(t.numel() == 0 || t.stride(dim - 1) == 1 || t.size(dim - 1) <= 1, name, ": ", what,
+              " must have unit stride along its last dim");
+}
+
+at::Tensor output_for(const c10::optional<at::Tensor>& out, const at::Tensor& q, int64_t d,
+                      const char* name) {
+  if (!out || !out->defined()) return at::empty({q.size(0), q.size(1), d}, q.options());
+  TORCH_CHECK(out->dim() == 3 && out->size(0) == q.size(0) && out->size(1) == q.size(1) &&
+                  out->size(2) == d && out->scalar_type() == q.scalar_type() &&
+                  out->device() == q.device(),
+              name, ": output must be [", q.size(0), ", ", q.size(1), ", ", d,
+              "] of q's dtype and device");
+  TORCH_CHECK(out->stride(2) == 1, name, ": output must have unit stride along its last dim");
+  return *out;
+}
+
+at::Tensor gqa_prompt_attention(const at::Tensor& q_in, const at::Tensor& k_in,
+                                const at::Tensor& v_in, const at::Tensor& cu_seqlens,
+                                int64_t max_seqlen, double scale, c10::optional<at::Tensor> out) {
+  const char* name = "gqa_prompt_attention";
+  TORCH_CHECK(q_in.dim() == 3 && k_in.dim() == 3 && v_in.dim() == 3, name,
+              ": q, k and v must be [tokens, heads, head_dim]");
+  TORCH_CHECK(q_in.is_cuda() && k_in.is_cuda() && v_in.is_cuda() && cu_seqlens.is_cuda(),
+              "All tensors must be on CUDA");
+  TORCH_CHECK(q_in.scalar_type() == at::kBFloat16 || q_in.scalar_type() == at::kHalf, name,
+              " supports bf16 and fp16 (got ", q_in.scalar_type(), ")");
+  TORCH_CHECK(k_in.scalar_type() == q_in.scalar_type() && v_in.scalar_type() == q_in.scalar_type() &&
+                  k_in.device() == q_in.device() && v_in.device() == q_in.device(),
+              name, ": q, k and v must share one dtype and device");
+  TORCH_CHECK(k_in.size(0) == q_in.size(0) && v_in.size(0) == q_in.size(0) &&
+                  k_in.size(1) == v_in.size(1) && k_in.size(2) == q_in.size(2),
+              name, ": token, head or head_dim mismatch");
+  check_ints(cu_seqlens, q_in, 1, name, "cu_seqlens");
+  TORCH_CHECK(cu_seqlens.numel() >= 1, name, ": cu_seqlens must have batch + 1 entries");
+  const at::Tensor q = heads_legal(q_in), k = heads_legal(k_in), v = heads_legal(v_in);
+  at::Tensor o = output_for(out, q, v.size(2), name);
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_rc(frn_gqa_prompt_attention(
+               dtype_code(q), q.data_ptr(), stride_or(q, 0), stride_or(q, 1), k.data_ptr(),
+               stride_or(k, 0), stride_or(k, 1), v.data_ptr(), stride_or(v, 0), stride_or(v, 1),
+               o.data_ptr(), stride_or(o, 0), stride_or(o, 1), cu_seqlens.data_ptr<int32_t>(),
+               cu_seqlens.numel() - 1, q.size(0), max_seqlen, q.size(1), k.size(1), q.size(2),
+               v.size(2), static_cast<float>(scale), stream_of(q)),
+           name);
+  return o;
+}
+
+frn_paged_kv paged_view(const at::Tensor& k_pages, const at::Tensor& v_pages,
+                        const at::Tensor& page_table, const at::Tensor& like, const char* name) {
+  TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes(), name,
+              ": pools must both be [num_pages, page_size, kv_heads, head_dim]");
+  TORCH_CHECK(k_pages.is_cuda() && v_pages.is_cuda() && page_table.is_cuda(),
+              "All tensors must be on CUDA");
+  TORCH_CHECK(k_pages.scalar_type() == like.scalar_type() &&
+                  v_pages.scalar_type() == like.scalar_type() &&
+                  k_pages.device() == like.device() && v_pages.device() == like.device(),
+              name, ": pools must share the new tensors' dtype and device");
+  TORCH_CHECK(dtype_code(like) >= 0, name, ": only fp32, fp16, bf16 supported");
+  TORCH_CHECK((k_pages.stride(3) == 1 && v_pages.stride(3) == 1) || k_pages.numel() == 0, name,
+              ": pools must have unit stride along head_dim");
+  check_ints(page_table, like, 2, name, "page_table");
+  frn_paged_kv c;
+  c.k = k_pages.data_ptr();
+  c.v = v_pages.data_ptr();
+  c.num_pages = k_pages.size(0);
+  c.page_size = k_pages.size(1);
+  c.num_kv_heads = k_pages.size(2);
+  c.head_dim = k_pages.size(3);
+  c.k_page_stride = stride_or(k_pages, 0);
+  c.k_token_stride = stride_or(k_pages, 1);
+  c.k_head_stride = stride_or(k_pages, 2);
+  c.v_page_stride = stride_or(v_pages, 0);
+  c.v_token_stride = stride_or(v_pages, 1);
+  c.v_head_stride = stride_or(v_pages, 2);
+  c.page_table = page_table.numel() ? page_table.data_ptr<int32_t>() : nullptr;
+  c.page_table_stride = stride_or(page_table, 0);
+  c.max_pages = page_table.size(1);
+  return c;
+}
+
+at::Tensor gqa_paged_decode(const at::Tensor& q_in, const at::Tensor& k_pages,
+                            const at::Tensor& v_pages, const at::Tensor& page_table,
+                            const at::Tensor& seq_lens, double scale,
+                            c10::optional<at::Tensor> out) {
+  const char* name = "gqa_paged_decode";
+  TORCH_CHECK(q_in.dim() == 3, name, ": q must be [batch, heads, head_dim]");
+  TORCH_CHECK(q_in.is_cuda() && seq_lens.is_cuda(), "All tensors must be on CUDA");
+  const frn_paged_kv c = paged_view(k_pages, v_pages, page_table, q_in, name);
+  check_ints(seq_lens, q_in, 1, name, "seq_lens");
+  TORCH_CHECK(q_in.size(2) == c.head_dim, name, ": head_dim mismatch");
+  TORCH_CHECK(seq_lens.numel() == q_in.size(0) && page_table.size(0) == q_in.size(0), name,
+              ": seq_lens and page_table must have an entry per sequence");
+  const at::Tensor q = heads_legal(q_in);
+  at::Tensor o = output_for(out, q, c.head_dim, name);
+  if (q.size(0) == 0) return o;
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int dt = dtype_code(q);
+  const size_t need = frn_gqa_paged_decode_workspace_size(dt, q.size(0), q.size(1), c.num_kv_heads,
+                                                          c.head_dim, c.page_size, c.max_pages);
+  const at::Tensor ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
+  check_rc(frn_gqa_paged_decode_attention(dt, q.data_ptr(), stride_or(q, 0), stride_or(q, 1), &c,
+                                          seq_lens.data_ptr<int32_t>(), o.data_ptr(),
+                                          stride_or(o, 0), stride_or(o, 1), q.size(0), q.size(1),
+                                          static_cast<float>(scale), ws.data_ptr(), need,
+                                          stream_of(q)),
+           name);
+  return o;
+}
+
+void kv_cache_append(const at::Tensor& k_in, const at::Tensor& v_in, at::Tensor k_pages,
+                     at::Tensor v_pages, const at::Tensor& page_table,
+                     const at::Tensor& start_lens, const c10::optional<at::Tensor>& cu_seqlens) {
+  const char* name = "kv_cache_append";
+  TORCH_CHECK(k_in.dim() == 3 && k_in.sizes() == v_in.sizes(), name,
+              ": k and v must both be [tokens, kv_heads, head_dim]");
+  TORCH_CHECK(k_in.is_cuda() && v_in.is_cuda() && start_lens.is_cuda(),
+              "All tensors must be on CUDA");
+  TORCH_CHECK(v_in.scalar_type() == k_in.scalar_type() && v_in.device() == k_in.device(), name,
+              ": k and v must share one dtype and device");
+  const frn_paged_kv c = paged_view(k_pages, v_pages, page_table, k_in, name);
+  TORCH_CHECK(k_in.size(1) == c.num_kv_heads && k_in.size(2) == c.head_dim, name,
+              ": kv_heads or head_dim mismatch");
+  check_ints(start_lens, k_in, 1, name, "start_lens");
+  const int64_t batch = start_lens.numel();
+  TORCH_CHECK(page_table.size(0) == batch, name,
+              ": start_lens and page_table must have an entry per sequence");
+  const int32_t* cu = nullptr;
+  if (cu_seqlens && cu_seqlens->defined()) {
+    TORCH_CHECK(cu_seqlens->is_cuda(), "All tensors must be on CUDA");
+    check_ints(*cu_seqlens, k_in, 1, name, "cu_seqlens");
+    TORCH_CHECK(cu_seqlens->numel() == batch + 1, name, ": cu_seqlens must have batch + 1 entries");
+    cu = cu_seqlens->data_ptr<int32_t>();
+  }
+  const at::Tensor k = heads_legal(k_in), v = heads_legal(v_in);
+  const c10::cuda::CUDAGuard guard(k.device());
+  check_rc(frn_kv_cache_append(dtype_code(k), k.data_ptr(), stride_or(k, 0), stride_or(k, 1),
+                               v.data_ptr(), stride_or(v, 0), stride_or(v, 1), &c,
+                               start_lens.data_ptr<int32_t>(), cu, batch, k.size(0),
+                               stream_of(k)),
+           name);
+}
+
+void kv_pages_copy(const std::vector<at::Tensor>& pools, const std::vector<int64_t>& src,
+                   const std::vector<int64_t>& dst) {
+  const char* name = "kv_pages_copy";
+  TORCH_CHECK(src.size() == dst.size(), name, ": src and dst must have the same length");
+  if (pools.empty() || src.empty()) return;
+  const at::Tensor& first = pools[0];
+  TORCH_CHECK(first.dim() >= 2, name, ": a pool must be [num_pages, ...]");
+  std::vector<void*> ptrs;
+  for (const at::Tensor& p : pools) {
+    TORCH_CHECK(p.is_cuda(), "All tensors must be on CUDA");
+    TORCH_CHECK(p.sizes() == first.sizes() && p.strides() == first.strides() &&
+                    p.element_size() == first.element_size() && p.device() == first.device(),
+                name, ": pools must share shape, strides, element size and device");
+    ptrs.push_back(p.data_ptr());
+  }
+  TORCH_CHECK(first.size(0) == 0 || first.select(0, 0).is_non_overlapping_and_dense(), name,
+              ": a page must be one dense block");
+  std::vector<int32_t> from, to;
+  for (size_t i = 0; i < src.size(); ++i) {
+    TORCH_CHECK(src[i] >= 0 && src[i] < first.size(0) && dst[i] >= 0 && dst[i] < first.size(0),
+                name, ": copy ", i, ": page ", src[i], " -> ", dst[i], " outside the ",
+                first.size(0), " pages");
+    from.push_back(static_cast<int32_t>(src[i]));
+    to.push_back(static_cast<int32_t>(dst[i]));
+  }
+  const int64_t es = first.element_size();
+  const c10::cuda::CUDAGuard guard(first.device());
+  check_rc(frn_kv_pages_copy(ptrs.data(), static_cast<int64_t>(ptrs.size()), first.size(0),
+                             first.numel() / first.size(0) * es, stride_or(first, 0) * es,
+                             from.data(), to.data(), static_cast<int64_t>(from.size()),
+                             stream_of(first)),
+           name);
+}
+
 void rmsnorm_swiglu_impl(const at::Tensor& x, const at::Tensor& raw_output, at::Tensor& output,
                          const at::Tensor& b_new, int64_t h, int64_t intermediate, double eps,
                          int threads, const char* name) {
@@ -430,6 +632,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "Decode-step GQA attention into output (context split across SMs)", py::arg("q"),
         py::arg("k_cache"), py::arg("v_cache"), py::arg("output"), py::arg("group_size"),
         py::arg("scale"));
+  m.def("gqa_prompt_attention", &gqa_prompt_attention,
+        "Causal GQA attention over packed prompts: q [T, Hq, D], k / v [T, Hkv, D] -> [T, Hq, Dv]",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu_seqlens"), py::arg("max_seqlen"),
+        py::arg("scale"), py::arg("out") = py::none());
+  m.def("gqa_paged_decode", &gqa_paged_decode,
+        "Decode-step GQA attention over a paged cache: q [B, Hq, D], pools [P, page_size, Hkv, D]",
+        py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("scale"), py::arg("out") = py::none());
+  m.def("kv_cache_append", &kv_cache_append,
+        "Write k, v [T, Hkv, D] to their sequences' pages, after start_lens tokens",
+        py::arg("k"), py::arg("v"), py::arg("k_pages"), py::arg("v_pages"), py::arg("page_table"),
+        py::arg("start_lens"), py::arg("cu_seqlens") = py::none());
+  m.def("kv_pages_copy", &kv_pages_copy,
+        "Copy pages src[i] -> dst[i] within every pool, one launch", py::arg("pools"),
+        py::arg("src"), py::arg("dst"));
   m.def("rmsnorm_swiglu", &rmsnorm_swiglu,
         "RMSNorm + SwiGLU of a [gate | up] GEMM output into output (256 threads per row)",
         py::arg("x"), py::arg("raw_output"), py::arg("output"), py::arg("b_new"), py::arg("h"),

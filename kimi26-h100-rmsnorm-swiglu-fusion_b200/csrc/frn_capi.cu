@@ -359,6 +359,218 @@ int frn_gqa_decode_attention_noalloc(int dtype, const void* q, const void* k_cac
   return run_gqa_decode(g, S, static_cast<cudaStream_t>(stream));
 }
 
+// A stride between rows of `row` elements: multiples of 16 bytes, no overlap.
+static bool legal_stride(int64_t stride, int64_t row, int es) {
+  return stride >= row && (stride * es) % 16 == 0;
+}
+
+int frn_gqa_prompt_attention(int dtype, const void* q, int64_t q_token_stride,
+                             int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                             int64_t v_head_stride, void* out, int64_t out_token_stride,
+                             int64_t out_head_stride, const int32_t* cu_seqlens, int64_t batch,
+                             int64_t tokens, int64_t max_seqlen, int64_t num_q_heads,
+                             int64_t num_kv_heads, int64_t head_dim_qk, int64_t head_dim_v,
+                             float scale, void* stream) {
+  if (dtype != FRN_DTYPE_F16 && dtype != FRN_DTYPE_BF16)
+    return set_error(FRN_ERR_UNSUPPORTED, "prompt attention supports fp16 and bf16 (dtype %d)",
+                     dtype);
+  if (batch < 0 || tokens < 0 || max_seqlen < 0 || num_q_heads <= 0 || num_kv_heads <= 0)
+    return set_error(FRN_ERR_INVALID_ARGUMENT,
+                     "bad shape batch=%lld tokens=%lld max_seqlen=%lld q_heads=%lld kv_heads=%lld",
+                     (long long)batch, (long long)tokens, (long long)max_seqlen,
+                     (long long)num_q_heads, (long long)num_kv_heads);
+  if (!((head_dim_qk == 64 && head_dim_v == 64) || (head_dim_qk == 128 && head_dim_v == 128) ||
+        (head_dim_qk == 192 && head_dim_v == 128)))
+    return set_error(FRN_ERR_UNSUPPORTED,
+                     "head dims must be 64/64, 128/128 or 192/128 (got %lld/%lld)",
+                     (long long)head_dim_qk, (long long)head_dim_v);
+  if (num_q_heads % num_kv_heads || num_q_heads / num_kv_heads > 128)
+    return set_error(FRN_ERR_UNSUPPORTED,
+                     "num_q_heads must be a multiple of num_kv_heads with a group of at most 128");
+  if (tokens > 0x3fffffffLL || batch > 0xffffffLL || num_q_heads > 0xffffLL)
+    return set_error(FRN_ERR_UNSUPPORTED, "prompt attention dimensions too large");
+  if (batch == 0 || tokens == 0 || max_seqlen == 0) return FRN_OK;
+  if (!q || !k || !v || !out || !cu_seqlens)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "q, k, v, out and cu_seqlens must be non-null");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return set_error(FRN_ERR_MISALIGNED, "q, k, v and out must be 16-byte aligned");
+  if (!legal_stride(q_token_stride, head_dim_qk, 2) || !legal_stride(q_head_stride, head_dim_qk, 2) ||
+      !legal_stride(k_token_stride, head_dim_qk, 2) || !legal_stride(k_head_stride, head_dim_qk, 2) ||
+      !legal_stride(v_token_stride, head_dim_v, 2) || !legal_stride(v_head_stride, head_dim_v, 2) ||
+      !legal_stride(out_token_stride, head_dim_v, 2) || !legal_stride(out_head_stride, head_dim_v, 2))
+    return set_error(FRN_ERR_MISALIGNED,
+                     "token and head strides must be multiples of 8 elements, at least a head long");
+  const PromptProblem g{dtype, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride,
+                        v, v_token_stride, v_head_stride, out, out_token_stride, out_head_stride,
+                        cu_seqlens, batch, tokens, max_seqlen < tokens ? max_seqlen : tokens,
+                        num_q_heads, num_kv_heads, head_dim_qk, head_dim_v, scale};
+  return run_prompt_attention(g, static_cast<cudaStream_t>(stream));
+}
+
+// Checks a frn_paged_kv and turns it into what the kernels take.
+static int check_paged(int dtype, const frn_paged_kv* c, PagedView* v) {
+  if (dtype != FRN_DTYPE_F32 && dtype != FRN_DTYPE_F16 && dtype != FRN_DTYPE_BF16)
+    return set_error(FRN_ERR_UNSUPPORTED, "a paged cache holds fp32, fp16 or bf16 (dtype %d)",
+                     dtype);
+  if (!c) return set_error(FRN_ERR_INVALID_ARGUMENT, "cache must be non-null");
+  if (c->num_pages < 0 || c->page_size <= 0 || c->num_kv_heads <= 0 || c->max_pages < 0)
+    return set_error(FRN_ERR_INVALID_ARGUMENT,
+                     "bad cache num_pages=%lld page_size=%lld kv_heads=%lld max_pages=%lld",
+                     (long long)c->num_pages, (long long)c->page_size, (long long)c->num_kv_heads,
+                     (long long)c->max_pages);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return set_error(FRN_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %lld)",
+                     (long long)c->head_dim);
+  // Positions are 32-bit, with room for a tile past the last one.
+  if (c->num_pages > 0x7fffffffLL || c->num_kv_heads > 0xffffLL || c->page_size > 0x3fffffffLL ||
+      c->max_pages > 0x7fff0000LL / c->page_size)
+    return set_error(FRN_ERR_UNSUPPORTED, "cache dimensions too large");
+  if ((c->num_pages > 0 && (!c->k || !c->v)) || (c->max_pages > 0 && !c->page_table))
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "k, v and page_table must be non-null");
+  if (!aligned16(c->k) || !aligned16(c->v))
+    return set_error(FRN_ERR_MISALIGNED, "cache pools must be 16-byte aligned");
+  const int es = elem_bytes(dtype);
+  for (const int64_t s : {c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride,
+                          c->v_token_stride, c->v_head_stride})
+    if (!legal_stride(s, c->head_dim, es))
+      return set_error(FRN_ERR_MISALIGNED,
+                       "cache strides must be multiples of 16 bytes, at least a head long");
+  if (c->page_table_stride < c->max_pages)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "page_table_stride %lld < max_pages %lld",
+                     (long long)c->page_table_stride, (long long)c->max_pages);
+  *v = PagedView{c->k, c->v, c->num_pages, c->max_pages, static_cast<int32_t>(c->page_size),
+                 static_cast<int32_t>(c->num_kv_heads), static_cast<int32_t>(c->head_dim),
+                 c->k_page_stride, c->k_token_stride, c->k_head_stride, c->v_page_stride,
+                 c->v_token_stride, c->v_head_stride, c->page_table, c->page_table_stride};
+  return 0;
+}
+
+size_t frn_gqa_paged_decode_workspace_size(int dtype, int64_t batch, int64_t num_q_heads,
+                                           int64_t num_kv_heads, int64_t head_dim,
+                                           int64_t page_size, int64_t max_pages) {
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || page_size <= 0 ||
+      max_pages < 0 || max_pages > 0x7fff0000LL / page_size)
+    return 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = 0;
+  return paged_decode_workspace(dtype, batch, num_q_heads, num_kv_heads, head_dim,
+                                page_size * max_pages, sm_count(dev));
+}
+
+int frn_gqa_paged_decode_attention(int dtype, const void* q, int64_t q_batch_stride,
+                                   int64_t q_head_stride, const frn_paged_kv* cache,
+                                   const int32_t* seq_lens, void* out, int64_t out_batch_stride,
+                                   int64_t out_head_stride, int64_t batch, int64_t num_q_heads,
+                                   float scale, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  PagedView kv;
+  int rc = check_paged(dtype, cache, &kv);
+  if (rc) return rc;
+  if (batch < 0 || num_q_heads <= 0)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "bad shape batch=%lld q_heads=%lld",
+                     (long long)batch, (long long)num_q_heads);
+  if (num_q_heads % kv.num_kv_heads || num_q_heads / kv.num_kv_heads > 16)
+    return set_error(FRN_ERR_UNSUPPORTED,
+                     "num_q_heads must be a multiple of num_kv_heads with a group of at most 16");
+  if (batch > 65535)
+    return set_error(FRN_ERR_UNSUPPORTED, "batch must be at most 65535 (got %lld)",
+                     (long long)batch);
+  if (batch == 0) return FRN_OK;
+  if (!q || !out || !seq_lens)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "q, out and seq_lens must be non-null");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace))
+    return set_error(FRN_ERR_MISALIGNED, "q, out and workspace must be 16-byte aligned");
+  const int es = elem_bytes(dtype);
+  if (!legal_stride(q_batch_stride, kv.head_dim, es) || !legal_stride(q_head_stride, kv.head_dim, es) ||
+      !legal_stride(out_batch_stride, kv.head_dim, es) || !legal_stride(out_head_stride, kv.head_dim, es))
+    return set_error(FRN_ERR_MISALIGNED,
+                     "q and out strides must be multiples of 16 bytes, at least a head long");
+  const size_t need = frn_gqa_paged_decode_workspace_size(
+      dtype, batch, num_q_heads, kv.num_kv_heads, kv.head_dim, kv.page_size, kv.max_pages);
+  if (!workspace || workspace_bytes < need)
+    return set_error(FRN_ERR_WORKSPACE, "paged decode needs %zu bytes of workspace (got %zu)", need,
+                     workspace ? workspace_bytes : size_t(0));
+  const PagedDecodeProblem g{dtype, kv, q, q_batch_stride, q_head_stride, out, out_batch_stride,
+                             out_head_stride, seq_lens, batch, num_q_heads, scale, workspace};
+  return run_paged_decode(g, static_cast<cudaStream_t>(stream));
+}
+
+int frn_kv_cache_append(int dtype, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                        const frn_paged_kv* cache, const int32_t* start_lens,
+                        const int32_t* cu_seqlens, int64_t batch, int64_t tokens, void* stream) {
+  PagedView kv;
+  int rc = check_paged(dtype, cache, &kv);
+  if (rc) return rc;
+  if (batch < 0 || tokens < 0)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "bad shape batch=%lld tokens=%lld",
+                     (long long)batch, (long long)tokens);
+  if (batch > 0x7fffffffLL || tokens > 0x7fffffffLL)
+    return set_error(FRN_ERR_UNSUPPORTED, "append dimensions too large");
+  if (!cu_seqlens && batch != tokens)
+    return set_error(FRN_ERR_INVALID_ARGUMENT,
+                     "without cu_seqlens there is one token a sequence (%lld tokens, batch %lld)",
+                     (long long)tokens, (long long)batch);
+  if (batch == 0 || tokens == 0) return FRN_OK;
+  if (!k || !v || !start_lens)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "k, v and start_lens must be non-null");
+  if (!aligned16(k) || !aligned16(v))
+    return set_error(FRN_ERR_MISALIGNED, "k and v must be 16-byte aligned");
+  const int es = elem_bytes(dtype);
+  // Rows are only read here: they may overlap, but not be misaligned.
+  for (const int64_t s : {k_token_stride, k_head_stride, v_token_stride, v_head_stride})
+    if (s < 0 || (s * es) % 16)
+      return set_error(FRN_ERR_MISALIGNED, "k and v strides must be multiples of 16 bytes");
+  const KvAppendProblem a{dtype, kv, k, k_token_stride, k_head_stride, v, v_token_stride,
+                          v_head_stride, start_lens, cu_seqlens, batch, tokens};
+  return run_kv_append(a, static_cast<cudaStream_t>(stream));
+}
+
+int frn_kv_pages_copy(void* const* pools, int64_t npools, int64_t num_pages, int64_t page_bytes,
+                      int64_t page_stride_bytes, const int32_t* src, const int32_t* dst,
+                      int64_t npairs, void* stream) {
+  if (npools < 0 || npairs < 0 || num_pages < 0 || page_bytes <= 0)
+    return set_error(FRN_ERR_INVALID_ARGUMENT,
+                     "bad copy npools=%lld npairs=%lld num_pages=%lld page_bytes=%lld",
+                     (long long)npools, (long long)npairs, (long long)num_pages,
+                     (long long)page_bytes);
+  if (page_bytes > (int64_t(1) << 28) || num_pages > 0x7fffffffLL)
+    return set_error(FRN_ERR_UNSUPPORTED, "pages of at most 256 MiB, at most 2^31 - 1 of them");
+  if (page_bytes % 16 || page_stride_bytes % 16 || page_stride_bytes < page_bytes)
+    return set_error(FRN_ERR_MISALIGNED,
+                     "page size and stride must be multiples of 16 bytes, the stride no smaller");
+  if (npools == 0 || npairs == 0) return FRN_OK;
+  if (!pools || !src || !dst)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "pools, src and dst must be non-null");
+  for (int64_t i = 0; i < npools; ++i) {
+    if (!pools[i]) return set_error(FRN_ERR_INVALID_ARGUMENT, "pool %lld is null", (long long)i);
+    if (!aligned16(pools[i]))
+      return set_error(FRN_ERR_MISALIGNED, "pools must be 16-byte aligned");
+  }
+  // One bit a page: is it written?  Then no source may be.
+  uint8_t* written = static_cast<uint8_t*>(std::calloc(static_cast<size_t>(num_pages / 8 + 1), 1));
+  if (!written) return set_error(FRN_ERR_CUDA, "out of host memory");
+  int rc = FRN_OK;
+  for (int64_t i = 0; i < npairs && rc == FRN_OK; ++i) {
+    if (src[i] < 0 || src[i] >= num_pages || dst[i] < 0 || dst[i] >= num_pages) {
+      rc = set_error(FRN_ERR_INVALID_ARGUMENT, "copy %lld: page %d -> %d outside the %lld pages",
+                     (long long)i, src[i], dst[i], (long long)num_pages);
+    } else if (written[dst[i] >> 3] >> (dst[i] & 7) & 1) {
+      rc = set_error(FRN_ERR_INVALID_ARGUMENT, "page %d is the destination of two copies", dst[i]);
+    } else {
+      written[dst[i] >> 3] |= static_cast<uint8_t>(1u << (dst[i] & 7));
+    }
+  }
+  for (int64_t i = 0; i < npairs && rc == FRN_OK; ++i)
+    if (written[src[i] >> 3] >> (src[i] & 7) & 1)
+      rc = set_error(FRN_ERR_INVALID_ARGUMENT, "page %d is both a source and a destination", src[i]);
+  std::free(written);
+  if (rc) return rc;
+  return run_kv_pages_copy(pools, npools, page_bytes, page_stride_bytes, src, dst, npairs,
+                           static_cast<cudaStream_t>(stream));
+}
+
 size_t frn_fused_rmsnorm_linear_workspace_size(int dtype, int64_t M, int64_t N, int64_t K) {
   (void)dtype; (void)M; (void)N; (void)K;
   return 0;

@@ -139,6 +139,70 @@ int run_gqa_decode_mma(const GqaProblem& g, int splits, cudaStream_t s);
 int gqa_noalloc_scratch(int dev, void** ptr);
 size_t gqa_noalloc_scratch_bytes();
 
+// A paged key-value cache as the kernels take it (struct frn_paged_kv, checked
+// by the C ABI; strides in elements).
+struct PagedView {
+  void* k;
+  void* v;
+  int64_t num_pages, max_pages;  // pages of the pools; entries of a page_table row
+  int32_t page_size, num_kv_heads, head_dim;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const int32_t* page_table;
+  int64_t table_stride;
+};
+
+// Decode-step attention over a paged cache (frn_paged_decode.cu).
+struct PagedDecodeProblem {
+  int dtype;
+  PagedView kv;
+  const void* q;
+  int64_t q_batch_stride, q_head_stride;
+  void* out;
+  int64_t out_batch_stride, out_head_stride;
+  const int32_t* seq_lens;
+  int64_t batch, num_q_heads;
+  float scale;
+  void* workspace;
+};
+size_t paged_decode_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d,
+                              int64_t capacity, int sms);
+int run_paged_decode(const PagedDecodeProblem& g, cudaStream_t s);
+
+// Appending tokens to a paged cache, copying pages (frn_kv_cache.cu).
+struct KvAppendProblem {
+  int dtype;
+  PagedView kv;
+  const void* k;
+  int64_t k_token_stride, k_head_stride;
+  const void* v;
+  int64_t v_token_stride, v_head_stride;
+  const int32_t* start_lens;
+  const int32_t* cu_seqlens;  // null: one token per sequence
+  int64_t batch, tokens;
+};
+int run_kv_append(const KvAppendProblem& a, cudaStream_t s);
+int run_kv_pages_copy(void* const* pools, int64_t npools, int64_t page_bytes,
+                      int64_t page_stride_bytes, const int32_t* src, const int32_t* dst,
+                      int64_t npairs, cudaStream_t s);
+
+// Causal attention over packed prompts (frn_prompt_attention.cu).
+struct PromptProblem {
+  int dtype;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  const void* k;
+  int64_t k_token_stride, k_head_stride;
+  const void* v;
+  int64_t v_token_stride, v_head_stride;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  const int32_t* cu_seqlens;
+  int64_t batch, tokens, max_seqlen, Hq, Hkv, Dqk, Dv;
+  float scale;
+};
+int run_prompt_attention(const PromptProblem& g, cudaStream_t s);
+
 int run_rmsnorm_swiglu(int dtype, const void* x, int64_t xs, const void* raw, int64_t rs,
                        void* out, int64_t os, const void* b, int64_t rows, int64_t h,
                        int64_t inter, float eps, int threads, cudaStream_t s);

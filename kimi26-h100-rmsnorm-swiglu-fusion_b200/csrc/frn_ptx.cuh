@@ -16,6 +16,8 @@ namespace frn {
 extern __device__ uint32_t g_frn_device_error;
 
 constexpr uint32_t kDevErrWaitTimeout = 0x1u;
+constexpr uint32_t kDevErrBadPage = 0x2u;
+constexpr uint32_t kDevErrBadLength = 0x4u;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -41,6 +41,9 @@ CU_SOURCES = [
     "frn_normalize.cu",
     "frn_gqa_decode.cu",
     "frn_gqa_decode_mma.cu",
+    "frn_prompt_attention.cu",
+    "frn_paged_decode.cu",
+    "frn_kv_cache.cu",
 ]
 HEADERS = ["frn_ptx.cuh", "frn_internal.h", "frn_pair_common.cuh"]
 

@@ -25,6 +25,10 @@ FRN_DTYPE_F32 = 0
 FRN_DTYPE_F16 = 1
 FRN_DTYPE_BF16 = 2
 
+FRN_DEVERR_WAIT_TIMEOUT = 0x1
+FRN_DEVERR_BAD_PAGE = 0x2
+FRN_DEVERR_BAD_LENGTH = 0x4
+
 FRN_KERNEL_AUTO = 0
 FRN_KERNEL_TILE_N128 = 1
 FRN_KERNEL_TILE_N192 = 2
@@ -50,6 +54,16 @@ class W8Linear(ctypes.Structure):
                 ("wq", c_void_p), ("N", c_int64), ("wq_row_stride", c_int64),
                 ("w_scale", c_void_p), ("bias", c_void_p), ("out", c_void_p),
                 ("out_row_stride", c_int64)]
+
+
+class PagedKV(ctypes.Structure):
+    """struct frn_paged_kv of include/frn_b200.h."""
+    _fields_ = ([("k", c_void_p), ("v", c_void_p)]
+                + [(n, c_int64) for n in ("num_pages", "page_size", "num_kv_heads", "head_dim",
+                                          "k_page_stride", "k_token_stride", "k_head_stride",
+                                          "v_page_stride", "v_token_stride", "v_head_stride")]
+                + [("page_table", c_void_p), ("page_table_stride", c_int64),
+                   ("max_pages", c_int64)])
 
 
 PROTOTYPES = {
@@ -108,6 +122,27 @@ PROTOTYPES = {
         c_int,
         [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
          c_int64, c_float, c_void_p],
+    ),
+    "frn_gqa_prompt_attention": (
+        c_int,
+        [c_int] + [c_void_p, c_int64, c_int64] * 4
+        + [c_void_p] + [c_int64] * 7 + [c_float, c_void_p],
+    ),
+    "frn_gqa_paged_decode_workspace_size": (c_size_t, [c_int] + [c_int64] * 6),
+    "frn_gqa_paged_decode_attention": (
+        c_int,
+        [c_int, c_void_p, c_int64, c_int64, ctypes.POINTER(PagedKV), c_void_p, c_void_p, c_int64,
+         c_int64, c_int64, c_int64, c_float, c_void_p, c_size_t, c_void_p],
+    ),
+    "frn_kv_cache_append": (
+        c_int,
+        [c_int] + [c_void_p, c_int64, c_int64] * 2
+        + [ctypes.POINTER(PagedKV), c_void_p, c_void_p, c_int64, c_int64, c_void_p],
+    ),
+    "frn_kv_pages_copy": (
+        c_int,
+        [ctypes.POINTER(c_void_p), c_int64, c_int64, c_int64, c_int64, ctypes.POINTER(ctypes.c_int32),
+         ctypes.POINTER(ctypes.c_int32), c_int64, c_void_p],
     ),
     "frn_device_error": (c_int, [c_int, ctypes.POINTER(c_uint32), c_int]),
     "frn_selftest_wait_timeout": (c_int, [c_int, c_void_p]),
@@ -354,6 +389,85 @@ def gqa_decode_attention_noalloc(q, k_cache, v_cache, scale: float, out):
             B, Hq, Hkv, D, T, float(scale), _stream_ptr(q.device))
     check(rc, "frn_gqa_decode_attention_noalloc")
     return out
+
+
+def gqa_prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=None):
+    """Causal attention over packed prompts through the C ABI: q [T, Hq, Dqk],
+    k [T, Hkv, Dqk], v [T, Hkv, Dv], cu_seqlens int32 [B + 1] on the GPU;
+    returns out [T, Hq, Dv]."""
+    import torch
+
+    T, Hq, Dqk = q.shape
+    Hkv, Dv = v.shape[1], v.shape[2]
+    if out is None:
+        out = torch.empty(T, Hq, Dv, dtype=q.dtype, device=q.device)
+    with _on(q.device):
+        rc = lib().frn_gqa_prompt_attention(
+            _dtype_code(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+            k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), out.data_ptr(), out.stride(0),
+            out.stride(1), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, T, int(max_seqlen), Hq,
+            Hkv, Dqk, Dv, float(scale), _stream_ptr(q.device))
+    check(rc, "frn_gqa_prompt_attention")
+    return out
+
+
+def paged_kv(k_pages, v_pages, page_table) -> PagedKV:
+    """The struct frn_paged_kv of pools [P, page_size, Hkv, D] and a table [B, max_pages]."""
+    P, page_size, Hkv, D = k_pages.shape
+    return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), P, page_size, Hkv, D,
+                   k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), v_pages.stride(0),
+                   v_pages.stride(1), v_pages.stride(2), page_table.data_ptr(),
+                   page_table.stride(0), page_table.shape[1])
+
+
+def gqa_paged_decode_attention(q, k_pages, v_pages, page_table, seq_lens, scale: float, out=None,
+                               workspace=None):
+    """Decode-step GQA attention over a paged cache through the C ABI: q
+    [B, Hq, D], pools [P, page_size, Hkv, D], page_table int32 [B, max_pages]
+    and seq_lens int32 [B] on the GPU; returns out [B, Hq, D]."""
+    import torch
+
+    B, Hq, D = q.shape
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    cache = paged_kv(k_pages, v_pages, page_table)
+    with _on(q.device):
+        if workspace is None:
+            need = lib().frn_gqa_paged_decode_workspace_size(
+                _dtype_code(q), B, Hq, cache.num_kv_heads, D, cache.page_size, cache.max_pages)
+            workspace = torch.empty(int(need), dtype=torch.uint8, device=q.device)
+        rc = lib().frn_gqa_paged_decode_attention(
+            _dtype_code(q), q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(cache),
+            seq_lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), B, Hq, float(scale),
+            workspace.data_ptr(), workspace.numel(), _stream_ptr(q.device))
+    check(rc, "frn_gqa_paged_decode_attention")
+    return out
+
+
+def kv_cache_append(k, v, k_pages, v_pages, page_table, start_lens, cu_seqlens=None) -> None:
+    """Writes k, v [T, Hkv, D] to their sequences' pages through the C ABI."""
+    cache = paged_kv(k_pages, v_pages, page_table)
+    with _on(k.device):
+        rc = lib().frn_kv_cache_append(
+            _dtype_code(k), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+            v.stride(1), ctypes.byref(cache), start_lens.data_ptr(),
+            cu_seqlens.data_ptr() if cu_seqlens is not None else None, start_lens.numel(),
+            k.shape[0], _stream_ptr(k.device))
+    check(rc, "frn_kv_cache_append")
+
+
+def kv_pages_copy(pools, src, dst) -> None:
+    """Copies pages src[i] -> dst[i] in every pool [P, ...] through the C ABI."""
+    n = len(src)
+    assert len(dst) == n and all(p.shape == pools[0].shape for p in pools)
+    ptrs = (c_void_p * len(pools))(*[p.data_ptr() for p in pools])
+    first = pools[0]
+    es = first.element_size()
+    with _on(first.device):
+        rc = lib().frn_kv_pages_copy(
+            ptrs, len(pools), first.shape[0], first[0].numel() * es, first.stride(0) * es,
+            (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, _stream_ptr(first.device))
+    check(rc, "frn_kv_pages_copy")
 
 
 def selftest_wait_timeout(timeout_ms: int, stream=None) -> None:

@@ -1,0 +1,226 @@
+"""GPU parity of causal attention over packed prompts (frn_gqa_prompt_attention
+and its Python surface) against the fp64 CPU oracle."""
+import itertools
+
+import pytest
+import torch
+
+from oracle import serving_attention as orc
+from src import capi
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+
+
+def cumulate(lens):
+    return [0] + list(itertools.accumulate(lens))
+
+
+def make(lens, Hq, Hkv, Dqk, Dv, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    T = sum(lens)
+    q = torch.randn(T, Hq, Dqk, generator=g).to(dtype)
+    k = torch.randn(T, Hkv, Dqk, generator=g).to(dtype)
+    v = torch.randn(T, Hkv, Dv, generator=g).to(dtype)
+    return q, k, v, cumulate(lens)
+
+
+def run(q, k, v, cu, scale, longest=None, out=None):
+    lens = [b - a for a, b in zip(cu[:-1], cu[1:])]
+    got = capi.gqa_prompt_attention(
+        q.to(DEV), k.to(DEV), v.to(DEV), torch.tensor(cu, dtype=torch.int32, device=DEV),
+        max(lens + [0]) if longest is None else longest, scale, out=out)
+    torch.cuda.synchronize()
+    return got
+
+
+def check(lens, Hq, Hkv, Dqk, Dv, dtype=torch.bfloat16, seed=0, scale=None, change=None):
+    q, k, v, cu = make(lens, Hq, Hkv, Dqk, Dv, dtype, seed)
+    if change is not None:
+        change(q, k, v, cu)
+    scale = Dqk ** -0.5 if scale is None else scale
+    got = run(q, k, v, cu, scale)
+    ref, spread = orc.prompt_attention(q, k, v, cu, scale)
+    orc.assert_close(got, ref, spread)
+    assert capi.device_error(0) == 0
+
+
+LENS = [
+    [1],
+    [2, 1, 5],
+    [77],
+    [127, 128, 129],
+    [64, 0, 0, 65, 31, 1, 32, 33],
+    [300],
+    [513, 17],
+    list(range(1, 40)),
+]
+
+
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: "-".join(map(str, x[:6])))
+@pytest.mark.parametrize("heads", [(8, 2, 128, 128), (7, 1, 64, 64), (2, 2, 192, 128)],
+                         ids=lambda x: "x".join(map(str, x)))
+def test_lengths(lens, heads):
+    check(lens, *heads, seed=sum(lens))
+
+
+@pytest.mark.parametrize("heads", [(1, 1, 128, 128), (3, 1, 128, 128), (10, 2, 128, 128),
+                                   (16, 1, 128, 128), (32, 2, 64, 64), (71, 1, 64, 64),
+                                   (128, 1, 64, 64), (6, 3, 192, 128)],
+                         ids=lambda x: "x".join(map(str, x)))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_head_layouts(heads, dtype):
+    check([130, 3, 45], *heads, dtype=dtype, seed=7)
+
+
+@pytest.mark.parametrize("heads", [(4, 1, 128, 128), (2, 2, 192, 128), (2, 1, 64, 64)],
+                         ids=lambda x: "x".join(map(str, x)))
+def test_long_sequence(heads):
+    check([1411, 700], *heads, seed=9)
+
+
+@pytest.mark.parametrize("Dqk,Dv", [(128, 128), (64, 64), (192, 128)])
+def test_running_maximum(Dqk, Dv):
+    """Scores that grow along the sequence move the maximum at every step; large
+    ones put nearly all weight on one key."""
+    def grow(q, k, v, cu):
+        q[:, :, 0] = 8.0
+        k[:, :, 0] = torch.linspace(-60, 60, k.shape[0])[:, None].to(k.dtype)
+
+    def shrink(q, k, v, cu):
+        q[:, :, 0] = 8.0
+        k[:, :, 0] = torch.linspace(60, -60, k.shape[0])[:, None].to(k.dtype)
+
+    for change in (grow, shrink):
+        check([600], 2, 1, Dqk, Dv, seed=3, change=change)
+    check([300], 2, 1, Dqk, Dv, seed=4, scale=4.0)
+    check([300], 2, 1, Dqk, Dv, seed=5, scale=0.0)
+    check([300], 2, 1, Dqk, Dv, seed=6, scale=-0.1)
+
+
+@pytest.mark.parametrize("Dqk,Dv", [(128, 128), (64, 64), (192, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_later_tokens_have_no_effect(Dqk, Dv, bad):
+    """Row i does not see what lies in k and v after it, whatever it is: not in
+    its own sequence, not in the next one."""
+    lens = [130, 40, 300]
+    q, k, v, cu = make(lens, 4, 2, Dqk, Dv, seed=11)
+    scale = Dqk ** -0.5
+    ref, spread = orc.prompt_attention(q, k, v, cu, scale)
+    for at in (cu[1] - 1, cu[1], cu[2] + 1, cu[2] + 77, cu[3] - 2):
+        k2, v2 = k.clone(), v.clone()
+        k2[at, :, 3] = bad
+        v2[at, :, 5] = bad
+        got = run(q, k2, v2, cu, scale).double().cpu()
+        rows = torch.arange(cu[-1])
+        seq_end = next(e for e in cu[1:] if at < e)
+        clean = (rows < at) | (rows >= seq_end)
+        orc.assert_close(got[clean].to(q.dtype), ref[clean], spread[clean])
+
+
+def test_strided_views():
+    """q, k and v as views of one QKV projection, V the tail of a [nope | V]
+    block, heads before tokens; the output a view too."""
+    T, Hq, Hkv, D = 150, 4, 2, 128
+    lens, cu = [100, 50], [0, 100, 150]
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn(T, Hq + 2 * Hkv, D, generator=g).to(torch.bfloat16).to(DEV)
+    q, k, v = qkv[:, :Hq], qkv[:, Hq:Hq + Hkv], qkv[:, Hq + Hkv:]
+    ref, spread = orc.prompt_attention(q.cpu(), k.cpu(), v.cpu(), cu, 0.1)
+    out = torch.full((T, Hq, 2 * D), 7.0, dtype=torch.bfloat16, device=DEV)
+    run(q, k, v, cu, 0.1, out=out[..., D:])
+    orc.assert_close(out[..., D:], ref, spread)
+    assert (out[..., :D] == 7).all()
+    by_head = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    orc.assert_close(run(*by_head, cu, 0.1), ref, spread)
+
+    k = torch.randn(T, Hkv, 192, generator=g).to(torch.bfloat16)
+    kv = torch.randn(T, Hkv, 256, generator=g).to(torch.bfloat16)
+    q = torch.randn(T, Hq, 192, generator=g).to(torch.bfloat16)
+    ref, spread = orc.prompt_attention(q, k, kv[..., 128:], cu, 0.07)
+    orc.assert_close(run(q, k, kv.to(DEV)[..., 128:], cu, 0.07), ref, spread)
+
+
+def test_rows_of_no_sequence_are_left_alone():
+    q, k, v, _ = make([90], 4, 2, 128, 128, seed=5)
+    cu = [10, 40, 80]
+    out = torch.full((90, 4, 128), 3.0, dtype=q.dtype, device=DEV)
+    run(q, k, v, cu, 0.1, out=out)
+    ref, spread = orc.prompt_attention(q, k, v, cu, 0.1)
+    orc.assert_close(out[10:80], ref[10:80], spread[10:80])
+    assert (out[:10] == 3).all() and (out[80:] == 3).all()
+
+
+def test_limits_are_enforced():
+    """A boundary past the tokens or a sequence past max_seqlen is cut and reported."""
+    q, k, v, _ = make([300], 4, 2, 128, 128, seed=6)
+    for cu, longest, inside in (([0, 100, 400], 300, [0, 100, 300]), ([0, 300], 140, [0, 140])):
+        out = torch.full((300, 4, 128), 3.0, dtype=q.dtype, device=DEV)
+        run(q, k, v, cu, 0.1, longest=longest, out=out)
+        assert capi.device_error(0, clear=True) == capi.FRN_DEVERR_BAD_LENGTH
+        ref, spread = orc.prompt_attention(q, k, v, inside, 0.1)
+        n = inside[-1]
+        orc.assert_close(out[:n], ref[:n], spread[:n])
+        assert (out[n:] == 3).all()
+    assert capi.device_error(0) == 0
+
+
+def test_nothing_to_do():
+    q, k, v, _ = make([4], 4, 2, 128, 128)
+    out = torch.full((4, 4, 128), 3.0, dtype=q.dtype, device=DEV)
+    run(q, k, v, [0], 0.1, longest=4, out=out)
+    run(q, k, v, [0, 0, 0], 0.1, longest=4, out=out)
+    assert (out == 3).all()
+    assert run(q[:0], k[:0], v[:0], [0, 0], 0.1, longest=0).shape == (0, 4, 128)
+
+
+def test_streams_graphs_and_repeats():
+    q, k, v, cu = make([200, 333], 8, 2, 128, 128, seed=8)
+    first = run(q, k, v, cu, 0.09)
+    qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
+    cud = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = capi.gqa_prompt_attention(qd, kd, vd, cud, 333, 0.09)
+    side.synchronize()
+    assert torch.equal(first, again)
+    out = torch.empty_like(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        capi.gqa_prompt_attention(qd, kd, vd, cud, 333, 0.09, out=out)
+    qd.copy_(qd.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    ref, spread = orc.prompt_attention(qd.cpu(), k, v, cu, 0.09)
+    orc.assert_close(out, ref, spread)
+
+
+def test_python_surface():
+    from src.load_gqa_attention import gqa_attention_cuda as ops
+
+    q, k, v, cu = make([60, 9], 4, 2, 128, 128, seed=1)
+    ref, spread = orc.prompt_attention(q, k, v, cu, 0.1)
+    cud = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
+    orc.assert_close(ops.gqa_prompt_attention(qd, kd, vd, cud, 60, 0.1), ref, spread)
+    # Layouts the kernel cannot read are copied first.
+    odd = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (qd, kd, vd)]
+    orc.assert_close(ops.gqa_prompt_attention(*odd, cud, 60, 0.1), ref, spread)
+    one = kd[:, :1].expand(-1, 2, -1)
+    ref1, spread1 = orc.prompt_attention(q, one.cpu(), v, cu, 0.1)
+    orc.assert_close(ops.gqa_prompt_attention(qd, one, vd, cud, 60, 0.1), ref1, spread1)
+    shifted = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape)
+    shifted.copy_(qd)
+    orc.assert_close(ops.gqa_prompt_attention(shifted, kd, vd, cud, 60, 0.1), ref, spread)
+    for args, match in [((qd.float(), kd.float(), vd.float(), cud), "bf16 and fp16"),
+                        ((qd, kd.half(), vd, cud), "one dtype"),
+                        ((qd, kd[:5], vd, cud), "mismatch"),
+                        ((qd[:, :3], kd, vd, cud), "multiple of num_kv_heads"),
+                        ((qd, kd, vd[..., :64], cud), "head dims"),
+                        ((qd, kd, vd, cud.long()), "int32"),
+                        ((qd, kd, vd, cud.cpu()), "CUDA")]:
+        with pytest.raises(RuntimeError, match=match):
+            ops.gqa_prompt_attention(*args, 60, 0.1)
+    assert capi.device_error(0) == 0
