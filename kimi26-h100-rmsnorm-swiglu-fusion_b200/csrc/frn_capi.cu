@@ -126,6 +126,24 @@ int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
   return 0;
 }
 
+int encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
+                   const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                   const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn enc = get_encode_tiled();
+  if (!enc) return set_error(FRN_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+  const cuuint64_t st[3] = {strides[0], strides[1], strides[2]};
+  const cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, dt, 4, const_cast<void*>(base), d, st, bx, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(FRN_ERR_INVALID_ARGUMENT, "cuTensorMapEncodeTiled failed (%d) for a 4-D view",
+                     static_cast<int>(r));
+  return 0;
+}
+
 int sm_count(int device) {
   static int cache[kMaxDevices] = {0};
   if (device >= 0 && device < kMaxDevices && cache[device] > 0) return cache[device];

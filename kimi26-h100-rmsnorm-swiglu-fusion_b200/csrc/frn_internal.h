@@ -82,6 +82,10 @@ int encode_tmap_kblocks_3d(CUtensorMap* map, CUtensorMapDataType dt, const void*
 int encode_tmap_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
                    const uint64_t (&dims)[3], const uint64_t (&strides)[2],
                    const uint32_t (&box)[3], CUtensorMapSwizzle swizzle);
+// As encode_tmap_3d with one more dimension.
+int encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
+                   const uint64_t (&dims)[4], const uint64_t (&strides)[3],
+                   const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
 
 int sm_count(int device);
 // Bound on every in-kernel wait (FRN_WAIT_TIMEOUT_MS, default 2000 ms).

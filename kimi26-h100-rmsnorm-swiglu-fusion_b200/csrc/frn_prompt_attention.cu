@@ -6,6 +6,38 @@
 // for every token i of every sequence, j running over the tokens of the same
 // sequence; the sequences lie one after the other in the token dimension,
 // sequence b in rows [cu_seqlens[b], cu_seqlens[b + 1]).
+//
+// Work item: one KV head and 2 x TQ consecutive tokens of one sequence, TQ =
+// 128 / G.  All G query heads of a token share its keys, so (token, head)
+// pairs are the rows of the tile: row r of a 128-row tile is token r / G, head
+// r % G, which a 4-D TMA box (d, head of the group, KV head, token) delivers
+// in that order.  A short sequence thus fills its tiles G times as well, the
+// causal edge is G times finer, and every K/V tile serves two row tiles.
+// Items are numbered by falling length of their key range (the last blocks of
+// the longest sequences first), so that the device ends evenly.
+//
+// One CTA an SM takes items in that order, counting up in one round and down in
+// the next.  Two row tiles an item take turns on the tensor core:
+//   S_s = Q_s K_j^T   (128 rows x 128 keys, operands in shared memory)
+//   O_s += P_s V_j    (P_s from TMEM, where it overwrites S_s; V from shared
+//                      memory as it lies, keys being the slow dimension)
+// While one tile's S is exponentiated by its four warps (one row a thread, no
+// shuffles), the other tile's two products run.  MMAs are issued in the order
+// PV_0(j), S_0(j+1), PV_1(j), S_1(j+1): a completed S_s(j+1) implies a completed
+// PV_s(j), so the softmax warps need one barrier for both.  After a tile's last
+// PV comes its first S of the next item, so that the loads and first products
+// of an item run under the end of the last.
+//
+// Roles: warps 0-3 and 4-7 the softmax and output of tile 0 and 1, warp 8 loads
+// Q and K, warp 10 V (its ring may be full while a K tile is needed), warp 9
+// issues the MMAs, warp 11 finds the items.
+//
+// Softmax in base 2.  The maximum that scales the exponentials may lag the true
+// running maximum by up to 2^8 (kLag); O in TMEM is only rescaled, by the
+// warp whose rows need it, when the lag would grow beyond that.  The final
+// division makes the result independent of it.  P is rounded to the input type
+// for the second product; the row sums are of the unrounded values, in fp32.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -18,54 +50,747 @@
 
 namespace frn {
 
-// One warp per (token, query head): lanes hold the head dims, one key a step.
+constexpr int kPromptThreads = 384;
+constexpr int kRows = 128;   // rows of a tile
+constexpr int kKeys = 128;   // keys of a K/V tile
+constexpr int kItemSlots = 4;  // items that the scheduler is ahead
+constexpr float kLag = 8.f;  // log2 of the most that a probability may exceed 1
+
+// Two row tiles of one KV head: tokens from t0 on of the sequence in rows
+// [first, first + len).  len = 0: no more items.
+struct PromptItem {
+  int32_t first, len, t0, kvh;
+};
+
+template <int DQK, int DV>
+struct PromptCfg {
+  static constexpr int QH = DQK / 64, VH = DV / 64;  // 64-column halves (128-byte rows)
+  static constexpr int HALF = kKeys * 128;           // bytes of 128 rows x 64 columns
+  static constexpr int Q_BYTES = QH * HALF, K_BYTES = QH * HALF, V_BYTES = VH * HALF;
+  // As many K and V tiles as fit beside the two Q tiles.
+  static constexpr int NK = DQK == 192 ? 2 : DQK == 128 ? 3 : 5;
+  static constexpr int NV = DQK == 192 ? 1 : DQK == 128 ? 2 : 5;
+  static constexpr int OFF_K = 2 * Q_BYTES;
+  static constexpr int OFF_V = OFF_K + NK * K_BYTES;
+  static constexpr int OFF_BAR = OFF_V + NV * V_BYTES;
+  static constexpr int OFF_ITEMS = OFF_BAR + (10 + 2 * NK + 2 * NV + 2 * kItemSlots) * 8;
+  static constexpr int SMEM_BYTES = OFF_ITEMS + kItemSlots * 16 + 16 + 1024;
+  static_assert(SMEM_BYTES <= 232448, "shared memory of one SM");
+  // TMEM columns: S_0, S_1 (P_s in the first half of S_s), O_0, O_1.
+  static constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
+};
+
+struct PromptParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;  // elements
+  const int32_t* cu;
+  int32_t batch, tokens, max_seqlen, group, hkv, tq;
+  float qscale;     // |scale| * log2(e), never zero
+  uint32_t negate;  // scale < 0: S is computed with Q negated
+  uint64_t timeout_ns;
+};
+
+// D(tmem) (+)= A(tmem, 16-bit pairs) * B(smem).
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Descriptor of a B operand whose rows run along the contraction (keys): rows
+// of 64 columns (128 bytes, 128-byte swizzle), 8-row groups 1024 bytes apart
+// (stride offset), the next 64 columns `half_bytes` further (leading offset).
+__device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_byte_addr,
+                                                            uint32_t half_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_byte_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(half_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  d |= static_cast<uint64_t>(2u) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// Moves registers between the warpgroups: all warps of one execute it.
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m, uint64_t* bar,
+                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_addr(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_addr(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ float prompt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Rows [first, first + len) of sequence b, cut to the call's limits.
+__device__ __forceinline__ void sequence_of(const PromptParams& p, int b, int32_t& first,
+                                            int32_t& len) {
+  const int64_t a = p.cu[b], e = p.cu[b + 1];
+  int64_t a2 = a < 0 ? 0 : a, e2 = e > p.tokens ? p.tokens : e;
+  if (e2 - a2 > p.max_seqlen) e2 = a2 + p.max_seqlen;
+  if (a2 != a || e2 != e) atomicOr(&g_frn_device_error, kDevErrBadLength);
+  first = static_cast<int32_t>(a2);
+  len = e2 > a2 ? static_cast<int32_t>(e2 - a2) : 0;
+}
+
+
+// Item number `index` in the order of falling block number: whole warp, all
+// lanes get the result.  F(L) = items of block number >= L = sum_b max(0,
+// blocks_b - L) falls with L; the item's block is the largest L with F(L) >
+// index, and it is the (index - F(L + 1))-th sequence that has such a block.
+__device__ __forceinline__ bool find_item(const PromptParams& p, int64_t index, PromptItem& item) {
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int32_t per = 2 * p.tq;
+  int32_t first = 0, len = 0, most = 0;
+  auto blocks = [&](int b) {
+    if (b >= p.batch) return 0;
+    sequence_of(p, b, first, len);
+    return (len + per - 1) / per;
+  };
+  const int32_t own = blocks(lane);  // of the first 32 sequences
+  auto count = [&](int32_t level) {
+    int64_t n = own > level ? own - level : 0;
+    for (int b = lane + 32; b < p.batch; b += 32) {
+      const int32_t x = blocks(b);
+      n += x > level ? x - level : 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+  };
+  most = (p.max_seqlen + per - 1) / per;
+  int32_t level = 0, above;  // F(level) > index >= F(above)
+  if (p.batch == 1) {
+    const int32_t all = __shfl_sync(0xffffffffu, own, 0);
+    if (index >= all) return false;
+    level = all - 1 - static_cast<int32_t>(index);
+    above = level + 1;
+  } else {
+    if (count(0) <= index) return false;
+    above = most;
+    while (above - level > 1) {
+      const int32_t mid = (level + above) >> 1;
+      if (count(mid) > index) level = mid; else above = mid;
+    }
+  }
+  int64_t k = index - (p.batch == 1 ? index : count(level + 1));
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const bool has = blocks(b0 + lane) > level;
+    const uint32_t mask = __ballot_sync(0xffffffffu, has);
+    if (k < __popc(mask)) {
+      int src = 0;
+      uint32_t m = mask;
+      for (; k > 0; --k) m &= m - 1;
+      src = __ffs(m) - 1;
+      item.first = __shfl_sync(0xffffffffu, first, src);
+      item.len = __shfl_sync(0xffffffffu, len, src);
+      item.t0 = level * per;
+      return true;
+    }
+    k -= __popc(mask);
+  }
+  return false;
+}
+
+// Row `tok` of one query head by the definition, a key at a time: whole warp.
+// Only for rows whose product with V met a NaN or an infinity at a position
+// that the row does not see (zero weight times that is not zero).
 template <typename T, int DQK, int DV>
-__global__ void __launch_bounds__(128) prompt_attention_kernel(const PromptProblem p) {
+__device__ __noinline__ void exact_row(const PromptParams& p, int32_t first, int32_t tok, int kvh,
+                                       int head, int32_t covered) {
   constexpr int EQ = DQK / 32, EV = DV / 32;
   const int lane = static_cast<int>(threadIdx.x & 31);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= p.tokens * p.Hq) return;
-  const int64_t i = row / p.Hq, h = row % p.Hq, kvh = h / (p.Hq / p.Hkv);
-  int64_t first = -1;
-  for (int64_t b = 0; b < p.batch; ++b) {
-    const int64_t from = p.cu_seqlens[b], to = p.cu_seqlens[b + 1];
-    if (from < 0 || to > p.tokens || to - from > p.max_seqlen)
-      atomicOr(&g_frn_device_error, kDevErrBadLength);
-    if (from >= 0 && from <= i && i < to && i < from + p.max_seqlen) first = from;
-  }
-  if (first < 0) return;
-  const T* q = static_cast<const T*>(p.q) + i * p.q_token_stride + h * p.q_head_stride;
-  float qf[EQ], acc[EV];
+  const T* k = static_cast<const T*>(p.k) + first * p.k_token + kvh * p.k_head;
+  const T* v = static_cast<const T*>(p.v) + first * p.v_token + kvh * p.v_head;
+  bool met = false;
+  for (int32_t j = tok + 1; j < covered; ++j)
 #pragma unroll
-  for (int e = 0; e < EQ; ++e)
-    qf[e] = static_cast<float>(q[lane + 32 * e]) * p.scale * 1.4426950408889634f;
+    for (int e = 0; e < EV; ++e)
+      met |= !isfinite(static_cast<float>(v[j * p.v_token + lane + 32 * e]));
+  if (!__any_sync(0xffffffffu, met)) return;  // the row's own keys gave the value
+  const T* q = static_cast<const T*>(p.q) + (first + tok) * p.q_token + head * p.q_head;
+  const float qs = p.negate ? -p.qscale : p.qscale;
+  float qf[EQ], acc[EV], m = -FLT_MAX, l = 0.f;
+#pragma unroll
+  for (int e = 0; e < EQ; ++e) qf[e] = static_cast<float>(q[lane + 32 * e]) * qs;
 #pragma unroll
   for (int e = 0; e < EV; ++e) acc[e] = 0.f;
-  float m = -FLT_MAX, l = 0.f;
-  for (int64_t j = first; j <= i; ++j) {
-    const T* k = static_cast<const T*>(p.k) + j * p.k_token_stride + kvh * p.k_head_stride;
-    const T* v = static_cast<const T*>(p.v) + j * p.v_token_stride + kvh * p.v_head_stride;
-    float s = 0.f;
+  for (int32_t j = 0; j <= tok; ++j) {
+    float d = 0.f;
 #pragma unroll
-    for (int e = 0; e < EQ; ++e) s = fmaf(qf[e], static_cast<float>(k[lane + 32 * e]), s);
+    for (int e = 0; e < EQ; ++e)
+      d = fmaf(qf[e], static_cast<float>(k[j * p.k_token + lane + 32 * e]), d);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float m_new = fmaxf(m, s), c = exp2f(m - m_new), w = exp2f(s - m_new);
+    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    const float m_new = fmaxf(m, d), c = exp2f(m - m_new), w = exp2f(d - m_new);
     m = m_new;
     l = l * c + w;
+    bool lost = true;
 #pragma unroll
-    for (int e = 0; e < EV; ++e) acc[e] = fmaf(w, static_cast<float>(v[lane + 32 * e]), acc[e] * c);
+    for (int e = 0; e < EV; ++e) {
+      acc[e] = fmaf(w, static_cast<float>(v[j * p.v_token + lane + 32 * e]), acc[e] * c);
+      lost &= isnan(acc[e]);
+    }
+    if (__all_sync(0xffffffffu, lost)) break;  // NaN everywhere stays so
   }
-  T* out = static_cast<T*>(p.out) + i * p.out_token_stride + h * p.out_head_stride;
+  T* out = static_cast<T*>(p.out) + (first + tok) * p.out_token + head * p.out_head;
 #pragma unroll
   for (int e = 0; e < EV; ++e) out[lane + 32 * e] = static_cast<T>(acc[e] / l);
 }
 
 template <typename T, int DQK, int DV>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
+                            const __grid_constant__ CUtensorMap tmap_k,
+                            const __grid_constant__ CUtensorMap tmap_v,
+                            const __grid_constant__ PromptParams p) {
+  using C = PromptCfg<DQK, DV>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* k_full = q_empty + 2;
+  uint64_t* k_empty = k_full + C::NK;
+  uint64_t* v_full = k_empty + C::NK;
+  uint64_t* v_empty = v_full + C::NV;
+  uint64_t* s_full = v_empty + C::NV;
+  uint64_t* p_ready = s_full + 2;
+  uint64_t* o_full = p_ready + 2;
+  uint64_t* i_full = o_full + 2;
+  uint64_t* i_empty = i_full + kItemSlots;
+  PromptItem* items = reinterpret_cast<PromptItem*>(smem + C::OFF_ITEMS);
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(items + kItemSlots);
+  uint32_t* tmem_ptr = const_cast<uint32_t*>(abort_flag) + 1;
+
+  const int warp = static_cast<int>(warp_id_in_cta()), lane = static_cast<int>(threadIdx.x & 31);
+  const uint64_t to = p.timeout_ns;
+
+  if (warp == 8 && lane == 0) {
+    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_k);
+    prefetch_tmap(&tmap_v);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_ready[i], 4);  // the tile's softmax warps
+      mbar_init(&o_full[i], 1);
+    }
+    for (int i = 0; i < C::NK; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < C::NV; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < kItemSlots; ++i) {
+      mbar_init(&i_full[i], 1);
+      mbar_init(&i_empty[i], 11);  // every warp but the scheduler
+    }
+    *abort_flag = 0u;
+    fence_mbarrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_ptr, C::TM_COLS);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_ptr;
+  griddep_launch_dependents();
+  griddep_wait();
+
+  // The it-th item of this CTA, copied from the scheduler's slots.
+  auto next_item = [&](int32_t it, PromptItem& item) {
+    const int slot = it % kItemSlots;
+    if (!mbar_wait(&i_full[slot], static_cast<uint32_t>(it / kItemSlots) & 1u, abort_flag, to))
+      return false;
+    item = items[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&i_empty[slot]);
+    return item.len > 0;
+  };
+  // Row tile s of an item: tokens [t0 + s TQ, end), K/V tiles.
+  auto end_of = [&](const PromptItem& item, int s) {
+    return min(item.len, item.t0 + (s + 1) * p.tq);
+  };
+  auto tiles_of = [&](const PromptItem& item, int s) {
+    return item.t0 + s * p.tq < item.len ? (end_of(item, s) + kKeys - 1) / kKeys : 0;
+  };
+
+  if (warp >= 8) {
+    reg_dec<88>();
+    if (warp == 11) {
+      // ---- scheduler: round r takes the CTA's number, odd rounds count down
+      const int32_t ctas = static_cast<int32_t>(gridDim.x), me = static_cast<int32_t>(blockIdx.x);
+      for (int32_t it = 0;; ++it) {
+        const int64_t index = static_cast<int64_t>(it) * ctas + (it & 1 ? ctas - 1 - me : me);
+        PromptItem item;
+        const bool some = find_item(p, index / p.hkv, item);
+        item.kvh = static_cast<int32_t>(index % p.hkv);
+        if (!some) item.len = 0;  // the end
+        const int slot = it % kItemSlots;
+        if (!mbar_wait(&i_empty[slot], (static_cast<uint32_t>(it / kItemSlots) & 1u) ^ 1u,
+                       abort_flag, to))
+          break;
+        if (lane == 0) {
+          items[slot] = item;
+          mbar_arrive(&i_full[slot]);
+        }
+        __syncwarp();
+        if (!some) break;
+      }
+    } else if (warp == 8) {
+      // ---- loads of Q and K
+      const uint32_t q_bytes = static_cast<uint32_t>(C::QH * 128 * p.group * p.tq);
+      PromptItem item;
+      uint32_t nk = 0, nq[2] = {0, 0};
+      bool ok = true;
+      for (int32_t it = 0; ok && next_item(it, item); ++it) {
+        const int32_t n = max(tiles_of(item, 0), tiles_of(item, 1));
+        auto load_q = [&](int s) {
+          if (tiles_of(item, s) == 0) return;
+          ok = ok && mbar_wait(&q_empty[s], (nq[s] & 1u) ^ 1u, abort_flag, to);
+          ++nq[s];
+          if (ok && lane == 0) {
+            mbar_arrive_expect_tx(&q_full[s], q_bytes);
+            for (int h = 0; h < C::QH; ++h)
+              tma_load_4d(smem + s * C::Q_BYTES + h * C::HALF, &tmap_q, &q_full[s], h * 64, 0,
+                          item.kvh, item.first + item.t0 + s * p.tq);
+          }
+        };
+        auto load_k = [&](int32_t j) {
+          const uint32_t ks = nk % C::NK;
+          ok = ok && mbar_wait(&k_empty[ks], ((nk / C::NK) & 1u) ^ 1u, abort_flag, to);
+          ++nk;
+          if (ok && lane == 0) {
+            mbar_arrive_expect_tx(&k_full[ks], C::K_BYTES);
+            for (int h = 0; h < C::QH; ++h)
+              tma_load_3d(smem + C::OFF_K + ks * C::K_BYTES + h * C::HALF, &tmap_k, &k_full[ks],
+                          h * 64, item.kvh, item.first + j * kKeys);
+          }
+        };
+        load_q(0);
+        load_k(0);
+        load_q(1);
+        for (int32_t j = 1; j < n && ok; ++j) load_k(j);
+      }
+      if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
+    } else if (warp == 10) {
+      // ---- loads of V
+      PromptItem item;
+      uint32_t nv = 0;
+      bool ok = true;
+      for (int32_t it = 0; ok && next_item(it, item); ++it) {
+        const int32_t n = max(tiles_of(item, 0), tiles_of(item, 1));
+        for (int32_t j = 0; j < n && ok; ++j, ++nv) {
+          const uint32_t vs = nv % C::NV;
+          ok = mbar_wait(&v_empty[vs], ((nv / C::NV) & 1u) ^ 1u, abort_flag, to);
+          if (ok && lane == 0) {
+            mbar_arrive_expect_tx(&v_full[vs], C::V_BYTES);
+            for (int h = 0; h < C::VH; ++h)
+              tma_load_3d(smem + C::OFF_V + vs * C::V_BYTES + h * C::HALF, &tmap_v, &v_full[vs],
+                          h * 64, item.kvh, item.first + j * kKeys);
+          }
+        }
+      }
+      if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
+    } else {
+      // ---- MMAs: the whole warp runs the loop, one lane issues
+      const uint32_t base = smem_addr(smem);
+      constexpr uint32_t kFmt = Elem16<T>::kUmmaFormat;
+      const uint32_t idesc_pv = make_idesc_f16(kFmt, kRows, DV) | (1u << 16);  // B along keys
+      uint32_t nk = 0, nv = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // K tiles before the item; waits
+      bool ok = true;
+      // Keys of tile j that row tile s can see, in whole MMA steps of 16.
+      auto steps = [&](const PromptItem& x, int s, int32_t j) {
+        return (min(kKeys, end_of(x, s) - j * kKeys) + 15) / 16;
+      };
+      // S_s(j) of item x, whose K tiles start at number k0.
+      auto qk = [&](const PromptItem& x, int s, int32_t j, uint32_t k0) {
+        if (j == 0) ok = ok && mbar_wait(&q_full[s], nq[s]++ & 1u, abort_flag, to);
+        const uint32_t ks = (k0 + j) % C::NK;
+        ok = ok && mbar_wait(&k_full[ks], ((k0 + j) / C::NK) & 1u, abort_flag, to);
+        if (ok && lane == 0) {
+          const uint32_t idesc =
+              make_idesc_f16(kFmt, kRows, 16u * steps(x, s, j)) | (p.negate << 13);
+          const uint64_t qd = make_smem_desc_k_sw128(base + s * C::Q_BYTES);
+          const uint64_t kd = make_smem_desc_k_sw128(base + C::OFF_K + ks * C::K_BYTES);
+#pragma unroll
+          for (int i = 0; i < DQK / 16; ++i) {
+            const uint32_t off = ((i / 4) * C::HALF + (i % 4) * 32) >> 4;
+            umma_f16_ss(tmem + C::TM_S + s * 128, qd + off, kd + off, idesc, i > 0);
+          }
+          umma_commit(&s_full[s]);
+          const int32_t mine = tiles_of(x, s), other = tiles_of(x, s ^ 1);
+          if (j + 1 == mine) umma_commit(&q_empty[s]);
+          // The K tile's last reader is row tile 1, or 0 where 1 has no such tile.
+          if (s == 1 || j >= other) umma_commit(&k_empty[ks]);
+        }
+        __syncwarp();
+      };
+      PromptItem item, next;
+      bool some = next_item(0, item);
+      for (int s = 0; s < 2 && some && ok; ++s)
+        if (tiles_of(item, s) > 0) qk(item, s, 0, 0);
+      for (int32_t it = 0; some && ok; ++it) {
+        const int32_t nt0 = tiles_of(item, 0), nt1 = tiles_of(item, 1), n = max(nt0, nt1);
+        bool more = false, asked = false;
+        for (int32_t j = 0; j < n && ok; ++j, ++nv) {
+          const uint32_t vs = nv % C::NV;
+          ok = mbar_wait(&v_full[vs], (nv / C::NV) & 1u, abort_flag, to);
+          if (!ok) break;
+          const int32_t left = item.len - j * kKeys;
+          if (left < kKeys && (left & 15)) {
+            // The last MMA step reaches past the sequence: what lies there has
+            // weight zero, but zero times a NaN or infinity is not zero.
+            const int rows = 16 - (left & 15);
+            for (int i = lane; i < rows * 8 * C::VH; i += 32) {
+              const int r = left + i / (8 * C::VH), c = i % (8 * C::VH);
+              st_shared_v4(base + C::OFF_V + vs * C::V_BYTES + (c / 8) * C::HALF + r * 128 +
+                               (c % 8) * 16,
+                           0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          const uint64_t vd = make_smem_desc_mn_sw128(base + C::OFF_V + vs * C::V_BYTES, C::HALF);
+#pragma unroll 1
+          for (int s = 0; s < 2 && ok; ++s) {
+            const int32_t nt = s ? nt1 : nt0;
+            if (j < nt) {
+              ok = mbar_wait(&p_ready[s], np[s]++ & 1u, abort_flag, to);
+              if (!ok) break;
+              tc_fence_after();
+              if (lane == 0) {
+                const int m = steps(item, s, j);
+#pragma unroll
+                for (int i = 0; i < kKeys / 16; ++i)
+                  if (i < m)
+                    umma_f16_ts(tmem + C::TM_O + s * DV, tmem + C::TM_S + s * 128 + i * 8,
+                                vd + ((i * 2048) >> 4), idesc_pv, j > 0 || i > 0);
+                if (j + 1 == nt) umma_commit(&o_full[s]);
+              }
+              __syncwarp();
+            }
+            if (s == 1 ? j < nt1 : j >= nt1) {  // the V tile's last reader
+              if (lane == 0) umma_commit(&v_empty[vs]);
+              __syncwarp();
+            }
+            if (j + 1 < nt) {
+              qk(item, s, j + 1, nk);
+            } else if (j + 1 == (nt > 0 ? nt : n)) {
+              // Row tile s is done with this item: its first product of the
+              // next.  (A tile without rows is done at the end: before, the K
+              // ring may be full of this item.)
+              if (!asked) {
+                more = next_item(it + 1, next);
+                asked = true;
+              }
+              if (more && tiles_of(next, s) > 0) qk(next, s, 0, nk + n);
+            }
+          }
+        }
+        nk += n;
+        item = next;
+        some = more;
+      }
+    }
+  } else {
+    reg_inc<208>();
+    // ---- softmax: one row a thread
+    const int s = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tm_s = tmem + lanes + C::TM_S + s * 128;
+    const uint32_t tm_o = tmem + lanes + C::TM_O + s * DV;
+    uint32_t ns = 0, no = 0;  // waits so far on s_full and o_full
+    bool ok = true;
+    PromptItem item;
+    for (int32_t it = 0; ok && next_item(it, item); ++it) {
+      const int32_t nt = tiles_of(item, s);
+      if (nt == 0) continue;
+      const int32_t t0 = item.t0 + s * p.tq;
+      const int32_t tok = t0 + row_tok;  // position in the sequence
+      float m_used = 0.f, l = 0.f;
+      for (int32_t j = 0; j < nt; ++j) {
+        ok = mbar_wait(&s_full[s], ns++ & 1u, abort_flag, to);
+        if (!ok) break;
+        tc_fence_after();
+        float x[kKeys];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c * 32]));
+        tmem_ld_wait();
+        const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
+        if (j * kKeys + kKeys > t0 + 1) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (i >= seen) x[i] = -INFINITY;
+        }
+        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int i = 4; i < kKeys; i += 4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[i + e]);
+        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (j == 0) {
+          m_used = m_tile;
+        } else {
+          const bool grow = (m_tile - m_used) * p.qscale > kLag;
+          if (__any_sync(0xffffffffu, grow)) {
+            // PV(j - 1) is complete (see the order of issue) and PV(j) waits
+            // for p_ready, so O is this warp's to change.
+            const float m_new = fmaxf(m_used, m_tile);
+            const float c = prompt_exp2((m_used - m_new) * p.qscale);
+            m_used = m_new;
+            l *= c;
+#pragma unroll
+            for (int b = 0; b < DV; b += 16) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(tm_o + b, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+              tmem_st_32x32b_x16(tm_o + b, o);
+            }
+          }
+        }
+        const float2 scale2 = make_float2(p.qscale, p.qscale);
+        const float2 shift2 = make_float2(-m_used * p.qscale, -m_used * p.qscale);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float* a = &x[h * 64 + 2 * i];
+            const float2 y = fma2(make_float2(a[0], a[1]), scale2, shift2);
+            a[0] = prompt_exp2(y.x);
+            a[1] = prompt_exp2(y.y);
+            w[i] = float2_to_pair<T>(a[0], a[1]);
+          }
+          tmem_st_32x32b_x32(tm_s + h * 32, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[s]);
+        float2 sum[2] = {make_float2(x[0], x[1]), make_float2(x[2], x[3])};
+#pragma unroll
+        for (int i = 4; i < kKeys; i += 4) {
+          sum[0] = add2(sum[0], make_float2(x[i], x[i + 1]));
+          sum[1] = add2(sum[1], make_float2(x[i + 2], x[i + 3]));
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+      }
+      ok = ok && mbar_wait(&o_full[s], no++ & 1u, abort_flag, to);
+      if (!ok) break;
+      tc_fence_after();
+      const float inv = 1.f / l;
+      const int head = item.kvh * p.group + row_head;
+      T* out = static_cast<T*>(p.out) + static_cast<int64_t>(item.first + tok) * p.out_token +
+               static_cast<int64_t>(head) * p.out_head;
+      const bool live = row_tok < p.tq && tok < item.len;
+      bool odd = false;  // a value that is not finite
+#pragma unroll
+      for (int b = 0; b < DV; b += 32) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(tm_o + b, o);
+        tmem_ld_wait();
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          f[i] = __uint_as_float(o[i]) * inv;
+          odd |= !(fabsf(f[i]) <= FLT_MAX);
+        }
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(out + b + i) =
+                make_uint4(float2_to_pair<T>(f[i], f[i + 1]), float2_to_pair<T>(f[i + 2], f[i + 3]),
+                           float2_to_pair<T>(f[i + 4], f[i + 5]),
+                           float2_to_pair<T>(f[i + 6], f[i + 7]));
+        }
+      }
+      tc_fence_before();
+      for (uint32_t again = __ballot_sync(0xffffffffu, odd && live); again; again &= again - 1) {
+        const int src = __ffs(again) - 1;
+        // Keys that the row's MMAs covered, up to a whole step past its tile.
+        const int32_t covered = min(item.len, (end_of(item, s) + 15) / 16 * 16);
+        exact_row<T, DQK, DV>(p, item.first, __shfl_sync(0xffffffffu, tok, src), item.kvh,
+                              __shfl_sync(0xffffffffu, head, src), covered);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+template <typename T, int DQK, int DV>
 static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
-  prompt_attention_kernel<T, DQK, DV>
-      <<<static_cast<unsigned>((g.tokens * g.Hq + 3) / 4), 128, 0, stream>>>(g);
-  const cudaError_t e = cudaGetLastError();
+  using C = PromptCfg<DQK, DV>;
+  auto kern = prompt_attention_kernel<T, DQK, DV>;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_error("cudaGetDevice");
+  static bool ready[kMaxDevices] = {};
+  if (dev >= kMaxDevices || !ready[dev]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
+    if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(prompt attention)", e);
+    if (dev < kMaxDevices) ready[dev] = true;
+  }
+  const int64_t G = g.Hq / g.Hkv, tq = kRows / G;
+  const CUtensorMapDataType dt = Elem16<T>::kTmaType;
+  CUtensorMap tq_map, tk, tv;
+  {  // (d, head of the group, KV head, token)
+    const uint64_t dims[4] = {static_cast<uint64_t>(DQK), static_cast<uint64_t>(G),
+                              static_cast<uint64_t>(g.Hkv), static_cast<uint64_t>(g.tokens)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(g.q_head_stride) * 2,
+                                 static_cast<uint64_t>(G * g.q_head_stride) * 2,
+                                 static_cast<uint64_t>(g.q_token_stride) * 2};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(tq)};
+    const int rc = encode_tmap_4d(&tq_map, dt, g.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  const uint32_t box[3] = {64, 1, kKeys};
+  {
+    const uint64_t dims[3] = {static_cast<uint64_t>(DQK), static_cast<uint64_t>(g.Hkv),
+                              static_cast<uint64_t>(g.tokens)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(g.k_head_stride) * 2,
+                                 static_cast<uint64_t>(g.k_token_stride) * 2};
+    const int rc = encode_tmap_3d(&tk, dt, g.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  {
+    const uint64_t dims[3] = {static_cast<uint64_t>(DV), static_cast<uint64_t>(g.Hkv),
+                              static_cast<uint64_t>(g.tokens)};
+    const uint64_t strides[2] = {static_cast<uint64_t>(g.v_head_stride) * 2,
+                                 static_cast<uint64_t>(g.v_token_stride) * 2};
+    const int rc = encode_tmap_3d(&tv, dt, g.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  PromptParams p;
+  p.q = g.q;
+  p.k = g.k;
+  p.v = g.v;
+  p.q_token = g.q_token_stride;
+  p.q_head = g.q_head_stride;
+  p.k_token = g.k_token_stride;
+  p.k_head = g.k_head_stride;
+  p.v_token = g.v_token_stride;
+  p.v_head = g.v_head_stride;
+  p.out = g.out;
+  p.out_token = g.out_token_stride;
+  p.out_head = g.out_head_stride;
+  p.cu = g.cu_seqlens;
+  p.batch = static_cast<int32_t>(g.batch);
+  p.tokens = static_cast<int32_t>(g.tokens);
+  p.max_seqlen = static_cast<int32_t>(g.max_seqlen);
+  p.group = static_cast<int32_t>(G);
+  p.hkv = static_cast<int32_t>(g.Hkv);
+  p.tq = static_cast<int32_t>(tq);
+  p.negate = g.scale < 0.f ? 1u : 0u;
+  // A scale of zero (every key the same weight) still has to send the masked
+  // scores, -inf, to -inf: any factor far below the scores' rounding will do.
+  p.qscale = fabsf(g.scale) * 1.4426950408889634f;
+  if (!(p.qscale >= 1e-30f)) p.qscale = 1e-30f;
+  p.timeout_ns = wait_timeout_ns();
+  // No more items than the whole blocks of all tokens and one ragged one a
+  // sequence, nor than every sequence at its longest.
+  const int64_t per = 2 * tq;
+  int64_t items = g.tokens / per + g.batch;
+  const int64_t longest = g.batch * ((g.max_seqlen + per - 1) / per);
+  if (longest < items) items = longest;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t ctas = items * g.Hkv < sm_count(dev) ? items * g.Hkv : sm_count(dev);
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  cfg.blockDim = dim3(kPromptThreads);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tq_map, tk, tv, p);
   if (e != cudaSuccess) return set_cuda_error("launch prompt_attention", e);
   return 0;
 }

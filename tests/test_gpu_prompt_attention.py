@@ -80,6 +80,28 @@ def test_long_sequence(heads):
     check([1411, 700], *heads, seed=9)
 
 
+@pytest.mark.parametrize("heads", [(4, 4, 128, 128), (2, 2, 192, 128), (8, 4, 64, 64)],
+                         ids=lambda x: "x".join(map(str, x)))
+@pytest.mark.parametrize("length", [40, 128, 160, 257, 300, 390])
+def test_many_items(heads, length):
+    """Several work items for every SM, with one or two row tiles each."""
+    lens = [length, max(1, length // 2), length - 3, 0] * 60
+    q, k, v, cu = make(lens, *heads, seed=length)
+    got = run(q, k, v, cu, 0.1)
+    assert capi.device_error(0) == 0
+    some = [0, 1, 2, 117, 238]
+    for b in some:
+        a, e = cu[b], cu[b + 1]
+        ref, spread = orc.prompt_attention(q[a:e], k[a:e], v[a:e], [0, e - a], 0.1)
+        orc.assert_close(got[a:e], ref, spread)
+    # The others against the same sequence run alone (same tiles, same bits).
+    for b in range(len(lens)):
+        a, e = cu[b], cu[b + 1]
+        if b % 7 == 0 and e > a:
+            alone = run(q[a:e], k[a:e], v[a:e], [0, e - a], 0.1)
+            assert torch.equal(got[a:e], alone)
+
+
 @pytest.mark.parametrize("Dqk,Dv", [(128, 128), (64, 64), (192, 128)])
 def test_running_maximum(Dqk, Dv):
     """Scores that grow along the sequence move the maximum at every step; large
