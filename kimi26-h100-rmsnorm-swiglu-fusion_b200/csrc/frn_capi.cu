@@ -789,6 +789,9 @@ int frn_device_error(int device, uint32_t* flags, int clear) {
     const uint32_t zero = 0;
     e = cudaMemcpyToSymbol(g_frn_device_error, &zero, sizeof(uint32_t));
   }
+  uint32_t more = 0;
+  if (e == cudaSuccess) e = prompt_device_error(&more, clear != 0);
+  *flags |= more;
   if (device != prev) cudaSetDevice(prev);
   if (e != cudaSuccess) return set_cuda_error("reading the device error word", e);
   return FRN_OK;

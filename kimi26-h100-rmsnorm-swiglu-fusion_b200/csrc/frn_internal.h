@@ -206,6 +206,8 @@ struct PromptProblem {
   float scale;
 };
 int run_prompt_attention(const PromptProblem& g, cudaStream_t s);
+// Reads (and clears) that unit's own device error word, on the current device.
+cudaError_t prompt_device_error(uint32_t* flags, bool clear);
 
 int run_rmsnorm_swiglu(int dtype, const void* x, int64_t xs, const void* raw, int64_t rs,
                        void* out, int64_t os, const void* b, int64_t rows, int64_t h,

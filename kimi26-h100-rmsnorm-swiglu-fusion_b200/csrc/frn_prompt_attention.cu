@@ -22,15 +22,15 @@
 //   O_s += P_s V_j    (P_s from TMEM, where it overwrites S_s; V from shared
 //                      memory as it lies, keys being the slow dimension)
 // While one tile's S is exponentiated by its four warps (one row a thread, no
-// shuffles), the other tile's two products run.  MMAs are issued in the order
-// PV_0(j), S_0(j+1), PV_1(j), S_1(j+1): a completed S_s(j+1) implies a completed
-// PV_s(j), so the softmax warps need one barrier for both.  After a tile's last
-// PV comes its first S of the next item, so that the loads and first products
-// of an item run under the end of the last.
+// shuffles), the other tile's two products run.  The MMAs of a row tile are
+// issued by one thread in the order PV_s(j), S_s(j+1): a completed S_s(j+1)
+// implies a completed PV_s(j), so the softmax warps need one barrier for both.
+// After a tile's last PV comes its first S of the next item, so that the loads
+// and first products of an item run under the end of the last.
 //
-// Roles: warps 0-3 and 4-7 the softmax and output of tile 0 and 1, warp 8 loads
-// Q and K, warp 10 V (its ring may be full while a K tile is needed), warp 9
-// issues the MMAs, warp 11 finds the items.
+// Roles: warps 0-3 and 4-7 the softmax and output of tile 0 and 1, warps 9 and
+// 10 their MMAs, warp 8 loads Q and K, warp 11 finds the items and loads V (whose
+// ring may be full while a K tile is needed).
 //
 // Softmax in base 2.  The maximum that scales the exponentials may lag the true
 // running maximum by up to 2^8 (kLag); O in TMEM is only rescaled, by the
@@ -44,6 +44,7 @@
 
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include "frn_internal.h"
 #include "frn_ptx.cuh"
@@ -53,6 +54,8 @@ namespace frn {
 constexpr int kPromptThreads = 384;
 constexpr int kRows = 128;   // rows of a tile
 constexpr int kKeys = 128;   // keys of a K/V tile
+constexpr int kPolyEvery = 4;  // one pair of exponentials in so many by polynomial
+constexpr int kMost = 96;    // keys whose P is announced before the rest
 constexpr int kItemSlots = 4;  // items that the scheduler is ahead
 constexpr float kLag = 8.f;  // log2 of the most that a probability may exceed 1
 
@@ -73,7 +76,7 @@ struct PromptCfg {
   static constexpr int OFF_K = 2 * Q_BYTES;
   static constexpr int OFF_V = OFF_K + NK * K_BYTES;
   static constexpr int OFF_BAR = OFF_V + NV * V_BYTES;
-  static constexpr int OFF_ITEMS = OFF_BAR + (10 + 2 * NK + 2 * NV + 2 * kItemSlots) * 8;
+  static constexpr int OFF_ITEMS = OFF_BAR + (12 + 2 * NK + 2 * NV + 2 * kItemSlots) * 8;
   static constexpr int SMEM_BYTES = OFF_ITEMS + kItemSlots * 16 + 16 + 1024;
   static_assert(SMEM_BYTES <= 232448, "shared memory of one SM");
   // TMEM columns: S_0, S_1 (P_s in the first half of S_s), O_0, O_1.
@@ -118,20 +121,6 @@ __device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_byte_a
   return d;
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
-          taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -162,6 +151,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Moves registers between the warpgroups: all warps of one execute it.
 template <int N>
 __device__ __forceinline__ void reg_inc() {
@@ -185,9 +180,43 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+// True in one lane of a converged warp.  Unlike a test of the lane number this
+// tells the compiler that the branch is for a single thread, so that the MMA's
+// uniform operands need no loop over lanes (a PV of eight MMAs is issued in ...
+// cycles instead of 770).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 __device__ __forceinline__ float prompt_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^x by the polynomial units, two at a time: x = r + f, r the nearest integer
+// (the sum with 1.5 * 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by a
+// degree-4 polynomial fitted to the least relative error (4e-6; P is rounded to
+// 2^-9 or 2^-12), r added to the exponent.  The special-function unit gives 16
+// exponentials a clock and an SM, as many clocks for a tile as its two products
+// take; a share of them done here relieves it.  x <= 8; below -126 the result
+// stays at 2^-126.
+__device__ __forceinline__ float2 poly_exp2(float2 x) {
+  constexpr float kRound = 12582912.f;
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 r = add2(x, make_float2(kRound, kRound));
+  const float2 f = fma2(add2(r, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
+  float2 y = fma2(f, make_float2(0.00957010221f, 0.00957010221f), make_float2(0.0559178591f, 0.0559178591f));
+  y = fma2(f, y, make_float2(0.240247443f, 0.240247443f));
+  y = fma2(f, y, make_float2(0.693121791f, 0.693121791f));
+  y = fma2(f, y, make_float2(0.999999285f, 0.999999285f));
+  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23));
+  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23));
   return y;
 }
 
@@ -325,7 +354,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* v_empty = v_full + C::NV;
   uint64_t* s_full = v_empty + C::NV;
   uint64_t* p_ready = s_full + 2;
-  uint64_t* o_full = p_ready + 2;
+  uint64_t* p_most = p_ready + 2;
+  uint64_t* o_full = p_most + 2;
   uint64_t* i_full = o_full + 2;
   uint64_t* i_empty = i_full + kItemSlots;
   PromptItem* items = reinterpret_cast<PromptItem*>(smem + C::OFF_ITEMS);
@@ -344,19 +374,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_ready[i], 4);  // the tile's softmax warps
+      mbar_init(&p_most[i], 5);   // and the other tile's MMA warp, handing over
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < C::NK; ++i) {
       mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], 2);  // both MMA warps
     }
     for (int i = 0; i < C::NV; ++i) {
       mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], 2);
     }
     for (int i = 0; i < kItemSlots; ++i) {
       mbar_init(&i_full[i], 1);
-      mbar_init(&i_empty[i], 11);  // every warp but the scheduler
+      mbar_init(&i_empty[i], 12);  // every warp
     }
     *abort_flag = 0u;
     fence_mbarrier_init();
@@ -392,27 +423,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 
   if (warp >= 8) {
     reg_dec<88>();
-    if (warp == 11) {
-      // ---- scheduler: round r takes the CTA's number, odd rounds count down
-      const int32_t ctas = static_cast<int32_t>(gridDim.x), me = static_cast<int32_t>(blockIdx.x);
-      for (int32_t it = 0;; ++it) {
-        const int64_t index = static_cast<int64_t>(it) * ctas + (it & 1 ? ctas - 1 - me : me);
-        PromptItem item;
-        const bool some = find_item(p, index / p.hkv, item);
-        item.kvh = static_cast<int32_t>(index % p.hkv);
-        if (!some) item.len = 0;  // the end
-        const int slot = it % kItemSlots;
-        if (!mbar_wait(&i_empty[slot], (static_cast<uint32_t>(it / kItemSlots) & 1u) ^ 1u,
-                       abort_flag, to))
-          break;
-        if (lane == 0) {
-          items[slot] = item;
-          mbar_arrive(&i_full[slot]);
-        }
-        __syncwarp();
-        if (!some) break;
-      }
-    } else if (warp == 8) {
+    if (warp == 8) {
       // ---- loads of Q and K
       const uint32_t q_bytes = static_cast<uint32_t>(C::QH * 128 * p.group * p.tq);
       PromptItem item;
@@ -448,11 +459,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int32_t j = 1; j < n && ok; ++j) load_k(j);
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
-    } else if (warp == 10) {
-      // ---- loads of V
+    } else if (warp == 11) {
+      // ---- items, two ahead of their V loads, and loads of V.  Round r takes
+      // the CTA's number; odd rounds count down.
+      const int32_t ctas = static_cast<int32_t>(gridDim.x), me = static_cast<int32_t>(blockIdx.x);
+      bool ok = true, done = false;
+      auto publish = [&](int32_t it) {
+        if (done || !ok) return;
+        const int64_t index = static_cast<int64_t>(it) * ctas + (it & 1 ? ctas - 1 - me : me);
+        PromptItem item;
+        done = !find_item(p, index / p.hkv, item);
+        item.kvh = static_cast<int32_t>(index % p.hkv);
+        if (done) item.len = 0;  // the end
+        const int slot = it % kItemSlots;
+        ok = mbar_wait(&i_empty[slot], (static_cast<uint32_t>(it / kItemSlots) & 1u) ^ 1u,
+                       abort_flag, to);
+        if (ok && lane == 0) {
+          items[slot] = item;
+          mbar_arrive(&i_full[slot]);
+        }
+        __syncwarp();
+      };
       PromptItem item;
       uint32_t nv = 0;
-      bool ok = true;
+      publish(0);
+      publish(1);
       for (int32_t it = 0; ok && next_item(it, item); ++it) {
         const int32_t n = max(tiles_of(item, 0), tiles_of(item, 1));
         for (int32_t j = 0; j < n && ok; ++j, ++nv) {
@@ -464,108 +495,189 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               tma_load_3d(smem + C::OFF_V + vs * C::V_BYTES + h * C::HALF, &tmap_v, &v_full[vs],
                           h * 64, item.kvh, item.first + j * kKeys);
           }
+          if (j == 0) publish(it + 2);
         }
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
     } else {
-      // ---- MMAs: the whole warp runs the loop, one lane issues
+      // ---- MMAs of row tile s: the whole warp runs the loop, one lane issues.
+      // What lies between a P and the next S is on the critical path, and waiting
+      // for a barrier costs two MMAs' time even if it is complete: one warp for
+      // both row tiles left the tensor core idle a third of the time.  The warps
+      // take turns, a PV and the following S at a time: left alone they fall
+      // into step, both softmaxes together, then both products (18% slower).
+      // A K/V tile is released by both warps; one whose row tile does not reach
+      // it waits for it all the same, to count in the right phase.
+      const int s = warp - 9;
       const uint32_t base = smem_addr(smem);
       constexpr uint32_t kFmt = Elem16<T>::kUmmaFormat;
-      const uint32_t idesc_pv = make_idesc_f16(kFmt, kRows, DV) | (1u << 16);  // B along keys
-      uint32_t nk = 0, nv = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // K tiles before the item; waits
+      constexpr uint32_t kIdescPV = make_idesc_f16(kFmt, kRows, DV) | (1u << 16);  // B along keys
+      const uint32_t idesc_qk = make_idesc_f16(kFmt, kRows, 0) | (p.negate << 13);
+      const uint64_t qd = make_smem_desc_k_sw128(base + s * C::Q_BYTES);
+      const uint64_t kd0 = make_smem_desc_k_sw128(base + C::OFF_K);
+      const uint64_t vd0 = make_smem_desc_mn_sw128(base + C::OFF_V, C::HALF);
+      const uint32_t tm_s = tmem + C::TM_S + s * 128, tm_o = tmem + C::TM_O + s * DV;
+      uint32_t ks = 0, kp = 0, vs = 0, vp = 0, qp = 0, pp = 0;  // ring slots and parities
+      uint32_t mp = 0;
       bool ok = true;
-      // Keys of tile j that row tile s can see, in whole MMA steps of 16.
-      auto steps = [&](const PromptItem& x, int s, int32_t j) {
-        return (min(kKeys, end_of(x, s) - j * kKeys) + 15) / 16;
+      // MMA steps (16 keys) of the row tile's last K/V tile.
+      auto last_steps = [&](const PromptItem& x, int32_t nt) {
+        return static_cast<uint32_t>(end_of(x, s) - (nt - 1) * kKeys + 15) / 16u;
       };
-      // S_s(j) of item x, whose K tiles start at number k0.
-      auto qk = [&](const PromptItem& x, int s, int32_t j, uint32_t k0) {
-        if (j == 0) ok = ok && mbar_wait(&q_full[s], nq[s]++ & 1u, abort_flag, to);
-        const uint32_t ks = (k0 + j) % C::NK;
-        ok = ok && mbar_wait(&k_full[ks], ((k0 + j) / C::NK) & 1u, abort_flag, to);
-        if (ok && lane == 0) {
-          const uint32_t idesc =
-              make_idesc_f16(kFmt, kRows, 16u * steps(x, s, j)) | (p.negate << 13);
-          const uint64_t qd = make_smem_desc_k_sw128(base + s * C::Q_BYTES);
-          const uint64_t kd = make_smem_desc_k_sw128(base + C::OFF_K + ks * C::K_BYTES);
+      // The operands of an item's K tile j have arrived.
+      auto wait_qk = [&](int32_t j, int32_t nt) {
+        if (j == 0 && nt > 0) {
+          ok = ok && mbar_wait(&q_full[s], qp, abort_flag, to);
+          qp ^= 1u;
+        }
+        ok = ok && mbar_wait(&k_full[ks], kp, abort_flag, to);
+      };
+      // By one lane: S of that tile, if the row tile has it.
+      auto issue_qk = [&](int32_t j, int32_t nt, uint32_t ragged) {
+        if (j < nt) {
+          const bool last = j + 1 == nt;
+          const uint32_t idesc = idesc_qk | ((last ? ragged : 8u) << 18);  // N = 16 a step
+          const uint64_t kd = kd0 + ks * (C::K_BYTES >> 4);
 #pragma unroll
           for (int i = 0; i < DQK / 16; ++i) {
             const uint32_t off = ((i / 4) * C::HALF + (i % 4) * 32) >> 4;
-            umma_f16_ss(tmem + C::TM_S + s * 128, qd + off, kd + off, idesc, i > 0);
+            umma_f16_ss(tm_s, qd + off, kd + off, idesc, i > 0);
           }
           umma_commit(&s_full[s]);
-          const int32_t mine = tiles_of(x, s), other = tiles_of(x, s ^ 1);
-          if (j + 1 == mine) umma_commit(&q_empty[s]);
-          // The K tile's last reader is row tile 1, or 0 where 1 has no such tile.
-          if (s == 1 || j >= other) umma_commit(&k_empty[ks]);
+          umma_commit(&k_empty[ks]);
+          if (last) umma_commit(&q_empty[s]);
+        } else {
+          mbar_arrive(&k_empty[ks]);
         }
-        __syncwarp();
       };
+      auto next_k = [&]() {
+        if (++ks == C::NK) {
+          ks = 0;
+          kp ^= 1u;
+        }
+      };
+      // The turn, and most of P with it: one wait for both.  Where there is no P
+      // to wait for, this warp stands in for the softmax warps.
+      auto take_turn = [&](bool with_p) {
+        if (!with_p && lane < 4) mbar_arrive(&p_most[s]);
+        ok = ok && mbar_wait(&p_most[s], mp, abort_flag, to);
+        mp ^= 1u;
+      };
+      if (s == 0 && lane == 0) mbar_arrive(&p_most[0]);  // row tile 0 begins
       PromptItem item, next;
       bool some = next_item(0, item);
-      for (int s = 0; s < 2 && some && ok; ++s)
-        if (tiles_of(item, s) > 0) qk(item, s, 0, 0);
+      int32_t nt = 0, other = 0;
+      uint32_t ragged = 0;
+      if (some) {
+        nt = tiles_of(item, s);
+        other = tiles_of(item, s ^ 1);
+        ragged = last_steps(item, nt);
+        wait_qk(0, nt);
+        take_turn(false);
+        if (ok && elect_one()) {
+          issue_qk(0, nt, ragged);
+          mbar_arrive(&p_most[s ^ 1]);
+        }
+        __syncwarp();
+        next_k();
+      }
       for (int32_t it = 0; some && ok; ++it) {
-        const int32_t nt0 = tiles_of(item, 0), nt1 = tiles_of(item, 1), n = max(nt0, nt1);
-        bool more = false, asked = false;
-        for (int32_t j = 0; j < n && ok; ++j, ++nv) {
-          const uint32_t vs = nv % C::NV;
-          ok = mbar_wait(&v_full[vs], (nv / C::NV) & 1u, abort_flag, to);
-          if (!ok) break;
-          const int32_t left = item.len - j * kKeys;
-          if (left < kKeys && (left & 15)) {
-            // The last MMA step reaches past the sequence: what lies there has
-            // weight zero, but zero times a NaN or infinity is not zero.
-            const int rows = 16 - (left & 15);
-            for (int i = lane; i < rows * 8 * C::VH; i += 32) {
-              const int r = left + i / (8 * C::VH), c = i % (8 * C::VH);
-              st_shared_v4(base + C::OFF_V + vs * C::V_BYTES + (c / 8) * C::HALF + r * 128 +
-                               (c % 8) * 16,
-                           0, 0, 0, 0);
+        const int32_t n = max(nt, other);
+        bool more = false;
+        int32_t next_nt = 0, next_other = 0;
+        uint32_t next_ragged = 0;
+        for (int32_t j = 0; j < n && ok; ++j) {
+          // Everything else that PV(j) and what follows it need, before P.
+          bool follows = true;
+          if (j + 1 < n) {
+            wait_qk(j + 1, nt);
+          } else {
+            follows = more = next_item(it + 1, next);
+            if (more) {
+              next_nt = tiles_of(next, s);
+              next_other = tiles_of(next, s ^ 1);
+              next_ragged = last_steps(next, next_nt);
+              wait_qk(0, next_nt);
             }
-            fence_proxy_async_smem();
-            __syncwarp();
           }
-          const uint64_t vd = make_smem_desc_mn_sw128(base + C::OFF_V + vs * C::V_BYTES, C::HALF);
-#pragma unroll 1
-          for (int s = 0; s < 2 && ok; ++s) {
-            const int32_t nt = s ? nt1 : nt0;
-            if (j < nt) {
-              ok = mbar_wait(&p_ready[s], np[s]++ & 1u, abort_flag, to);
-              if (!ok) break;
-              tc_fence_after();
-              if (lane == 0) {
-                const int m = steps(item, s, j);
+          ok = ok && mbar_wait(&v_full[vs], vp, abort_flag, to);
+          if (!ok) break;
+          const bool here = j < nt, last = j + 1 == nt;
+          const uint32_t steps = last ? ragged : 8u;
+          const uint64_t vd = vd0 + vs * (C::V_BYTES >> 4);
+          if (here) {
+            const int32_t left = item.len - j * kKeys;
+            if (left < kKeys && (left & 15)) {
+              // The last MMA step reaches past the sequence: what lies there has
+              // weight zero, but zero times a NaN or infinity is not zero.
+              // (Both MMA warps may write these zeros.)
+              const int rows = 16 - (left & 15);
+              for (int i = lane; i < rows * 8 * C::VH; i += 32) {
+                const int r = left + i / (8 * C::VH), c = i % (8 * C::VH);
+                st_shared_v4(base + C::OFF_V + vs * C::V_BYTES + (c / 8) * C::HALF + r * 128 +
+                                 (c % 8) * 16,
+                             0, 0, 0, 0);
+              }
+              fence_proxy_async_smem();
+              __syncwarp();
+            }
+          }
+          take_turn(here);
+          if (!ok) break;
+          if (here) {
+            tc_fence_after();
+            if (elect_one()) {
+              if (steps == 8u) {
 #pragma unroll
-                for (int i = 0; i < kKeys / 16; ++i)
-                  if (i < m)
-                    umma_f16_ts(tmem + C::TM_O + s * DV, tmem + C::TM_S + s * 128 + i * 8,
-                                vd + ((i * 2048) >> 4), idesc_pv, j > 0 || i > 0);
-                if (j + 1 == nt) umma_commit(&o_full[s]);
+                for (int i = 0; i < kMost / 16; ++i)
+                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV,
+                              j > 0 || i > 0);
+              } else {
+#pragma unroll 1
+                for (int i = 0; i < min(kMost / 16, static_cast<int>(steps)); ++i)
+                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV,
+                              j > 0 || i > 0);
               }
-              __syncwarp();
             }
-            if (s == 1 ? j < nt1 : j >= nt1) {  // the V tile's last reader
-              if (lane == 0) umma_commit(&v_empty[vs]);
-              __syncwarp();
-            }
-            if (j + 1 < nt) {
-              qk(item, s, j + 1, nk);
-            } else if (j + 1 == (nt > 0 ? nt : n)) {
-              // Row tile s is done with this item: its first product of the
-              // next.  (A tile without rows is done at the end: before, the K
-              // ring may be full of this item.)
-              if (!asked) {
-                more = next_item(it + 1, next);
-                asked = true;
+            __syncwarp();
+            ok = mbar_wait(&p_ready[s], pp, abort_flag, to);
+            pp ^= 1u;
+            if (!ok) break;
+            tc_fence_after();
+          }
+          if (elect_one()) {
+            if (here) {
+              if (steps == 8u) {
+#pragma unroll
+                for (int i = kMost / 16; i < kKeys / 16; ++i)
+                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, 1u);
+              } else {
+#pragma unroll 1
+                for (int i = kMost / 16; i < static_cast<int>(steps); ++i)
+                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, 1u);
               }
-              if (more && tiles_of(next, s) > 0) qk(next, s, 0, nk + n);
+              if (last) umma_commit(&o_full[s]);
             }
+            if (follows) issue_qk(j + 1 < n ? j + 1 : 0, j + 1 < n ? nt : next_nt,
+                                  j + 1 < n ? ragged : next_ragged);
+            mbar_arrive(&p_most[s ^ 1]);
+            if (here)
+              umma_commit(&v_empty[vs]);
+            else
+              mbar_arrive(&v_empty[vs]);
+          }
+          __syncwarp();
+          if (follows) next_k();
+          if (++vs == C::NV) {
+            vs = 0;
+            vp ^= 1u;
           }
         }
-        nk += n;
         item = next;
         some = more;
+        nt = next_nt;
+        other = next_other;
+        ragged = next_ragged;
       }
     }
   } else {
@@ -595,66 +707,93 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int c = 0; c < 4; ++c)
           tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c * 32]));
         tmem_ld_wait();
-        const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
-        if (j * kKeys + kKeys > t0 + 1) {
+        float2 sum = make_float2(0.f, 0.f);
+        // exp2 of 32 scores, their P and their sum.
+        auto piece = [&](auto mixed, float* v, uint32_t (&w)[16]) {
+          const float2 scale2 = make_float2(p.qscale, p.qscale);
+          const float2 shift2 = make_float2(-m_used * p.qscale, -m_used * p.qscale);
+          float2 part[2];
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
-            if (i >= seen) x[i] = -INFINITY;
-        }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
+          for (int i = 0; i < 16; ++i) {
+            float2 y = fma2(make_float2(v[2 * i], v[2 * i + 1]), scale2, shift2);
+            if (decltype(mixed)::value && i % kPolyEvery == kPolyEvery - 1) {
+              y = poly_exp2(y);
+            } else {
+              y.x = prompt_exp2(y.x);
+              y.y = prompt_exp2(y.y);
+            }
+            w[i] = float2_to_pair<T>(y.x, y.y);
+            part[i & 1] = i < 2 ? y : add2(part[i & 1], y);
+          }
+          sum = add2(sum, add2(part[0], part[1]));
+        };
+        auto tile = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
+          // Masked scores must come out as zero, not as the least that the
+          // polynomial gives.
+          constexpr std::integral_constant<bool, !kMasked> mixed{};
+          if (kMasked) {
+            const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
 #pragma unroll
-        for (int i = 4; i < kKeys; i += 4)
+            for (int i = 0; i < kKeys; ++i)
+              if (i >= seen) x[i] = -INFINITY;
+          }
+          // The first piece goes ahead with the maximum so far, while the tile's
+          // own is found; rarely, it has to be done again.
+          uint32_t w[16];
+          if (j > 0) piece(mixed, x, w);
+          float mx[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[i + e]);
-        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if (j == 0) {
-          m_used = m_tile;
-        } else {
-          const bool grow = (m_tile - m_used) * p.qscale > kLag;
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(x[e], x[4 + e]);
+#pragma unroll
+          for (int i = 8; i < kKeys; i += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + 2 * e], x[i + 2 * e + 1]);
+          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool grow = j == 0 || (m_tile - m_used) * p.qscale > kLag;
           if (__any_sync(0xffffffffu, grow)) {
-            // PV(j - 1) is complete (see the order of issue) and PV(j) waits
-            // for p_ready, so O is this warp's to change.
-            const float m_new = fmaxf(m_used, m_tile);
-            const float c = prompt_exp2((m_used - m_new) * p.qscale);
-            m_used = m_new;
-            l *= c;
+            if (j == 0) {
+              m_used = m_tile;
+            } else {
+              // PV(j - 1) is complete (see the order of issue) and PV(j) waits
+              // for this P, so O is this warp's to change.
+              const float m_new = fmaxf(m_used, m_tile);
+              const float c = prompt_exp2((m_used - m_new) * p.qscale);
+              m_used = m_new;
+              l *= c;
 #pragma unroll
-            for (int b = 0; b < DV; b += 16) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(tm_o + b, o);
-              tmem_ld_wait();
+              for (int b = 0; b < DV; b += 16) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(tm_o + b, o);
+                tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
-              tmem_st_32x32b_x16(tm_o + b, o);
+                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+                tmem_st_32x32b_x16(tm_o + b, o);
+              }
+            }
+            sum = make_float2(0.f, 0.f);
+            piece(std::integral_constant<bool, false>{}, x, w);
+          }
+          // P in pieces of 32 keys; the MMA warp starts on the first ones while
+          // the last is computed.
+          tmem_st_32x32b_x16(tm_s, w);
+#pragma unroll
+          for (int h = 1; h < kKeys / 32; ++h) {
+            piece(mixed, x + h * 32, w);
+            tmem_st_32x32b_x16(tm_s + h * 16, w);
+            if (h == kMost / 32 - 1 || h == kKeys / 32 - 1) {
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(h == kKeys / 32 - 1 ? &p_ready[s] : &p_most[s]);
             }
           }
-        }
-        const float2 scale2 = make_float2(p.qscale, p.qscale);
-        const float2 shift2 = make_float2(-m_used * p.qscale, -m_used * p.qscale);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float* a = &x[h * 64 + 2 * i];
-            const float2 y = fma2(make_float2(a[0], a[1]), scale2, shift2);
-            a[0] = prompt_exp2(y.x);
-            a[1] = prompt_exp2(y.y);
-            w[i] = float2_to_pair<T>(a[0], a[1]);
-          }
-          tmem_st_32x32b_x32(tm_s + h * 32, w);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[s]);
-        float2 sum[2] = {make_float2(x[0], x[1]), make_float2(x[2], x[3])};
-#pragma unroll
-        for (int i = 4; i < kKeys; i += 4) {
-          sum[0] = add2(sum[0], make_float2(x[i], x[i + 1]));
-          sum[1] = add2(sum[1], make_float2(x[i + 2], x[i + 3]));
-        }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          l += sum.x + sum.y;
+        };
+        if (j * kKeys + kKeys > t0 + 1)
+          tile(std::integral_constant<bool, true>{});
+        else
+          tile(std::integral_constant<bool, false>{});
       }
       ok = ok && mbar_wait(&o_full[s], no++ & 1u, abort_flag, to);
       if (!ok) break;
@@ -800,6 +939,14 @@ static int launch_prompt_d(const PromptProblem& g, cudaStream_t s) {
   if (g.Dqk == 192) return launch_prompt<T, 192, 128>(g, s);
   if (g.Dqk == 128) return launch_prompt<T, 128, 128>(g, s);
   return launch_prompt<T, 64, 64>(g, s);
+}
+
+cudaError_t prompt_device_error(uint32_t* flags, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(flags, g_frn_device_error, sizeof(uint32_t));
+  const uint32_t zero = 0;
+  if (e == cudaSuccess && clear && *flags)
+    e = cudaMemcpyToSymbol(g_frn_device_error, &zero, sizeof(uint32_t));
+  return e;
 }
 
 int run_prompt_attention(const PromptProblem& g, cudaStream_t s) {

@@ -13,7 +13,13 @@ namespace frn {
 // Device-wide error word (see frn_device_error in include/frn_b200.h).  A
 // kernel whose bounded wait expires ORs a bit in here and winds down instead
 // of hanging the GPU.
+// A unit compiled without relocatable device code (where setmaxnreg would be
+// ignored) has a word of its own, which frn_device_error reads too.
+#ifdef __CUDACC_RDC__
 extern __device__ uint32_t g_frn_device_error;
+#else
+static __device__ uint32_t g_frn_device_error = 0u;
+#endif
 
 constexpr uint32_t kDevErrWaitTimeout = 0x1u;
 constexpr uint32_t kDevErrBadPage = 0x2u;

@@ -58,6 +58,10 @@ NVCC_FLAGS = ARCH_FLAGS + [
     f"-I{INCLUDE_DIR}",
 ]
 
+# Units without relocatable device code: ptxas ignores setmaxnreg in a unit that
+# others may be linked to on the device.
+NO_RDC_SOURCES = ["frn_prompt_attention.cu"]
+
 _lock = threading.Lock()
 _lib_handle = None
 _ext_module = None
@@ -95,7 +99,7 @@ def _lib_inputs():
 def _flags_key() -> str:
     # The include path is absolute; the tree may be copied elsewhere (another
     # machine, a scratch directory), so the stamp records it relative.
-    return " ".join(f.replace(REPO_DIR, "<repo>") for f in NVCC_FLAGS)
+    return " ".join([f.replace(REPO_DIR, "<repo>") for f in NVCC_FLAGS] + NO_RDC_SOURCES)
 
 
 @contextlib.contextmanager
@@ -133,7 +137,8 @@ def _build_library_locked(force: bool, verbose: bool) -> str:
 
     def compile_one(src):
         obj = os.path.join(obj_dir, os.path.splitext(src)[0] + ".o")
-        cmd = [nvcc] + NVCC_FLAGS + ["-c", os.path.join(CSRC_DIR, src), "-o", obj]
+        flags = [f for f in NVCC_FLAGS if f != "-rdc=true" or src not in NO_RDC_SOURCES]
+        cmd = [nvcc] + flags + ["-c", os.path.join(CSRC_DIR, src), "-o", obj]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         r = subprocess.run(cmd, capture_output=True, text=True)
