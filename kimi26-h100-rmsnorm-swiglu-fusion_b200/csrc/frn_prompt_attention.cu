@@ -54,8 +54,8 @@ namespace frn {
 constexpr int kPromptThreads = 384;
 constexpr int kRows = 128;   // rows of a tile
 constexpr int kKeys = 128;   // keys of a K/V tile
-constexpr int kPolyEvery = 4;  // one pair of exponentials in so many by polynomial
-constexpr int kMost = 96;    // keys whose P is announced before the rest
+constexpr int kLoadQK = 8, kMma = 9, kLoadV = 11;  // warps; 0-3 and 4-7: softmax
+constexpr int kMost = 96;        // keys whose P is announced before the rest
 constexpr int kItemSlots = 4;  // items that the scheduler is ahead
 constexpr float kLag = 8.f;  // log2 of the most that a probability may exceed 1
 
@@ -77,7 +77,7 @@ struct PromptCfg {
   static constexpr int OFF_V = OFF_K + NK * K_BYTES;
   static constexpr int OFF_BAR = OFF_V + NV * V_BYTES;
   static constexpr int OFF_ITEMS = OFF_BAR + (12 + 2 * NK + 2 * NV + 2 * kItemSlots) * 8;
-  static constexpr int SMEM_BYTES = OFF_ITEMS + kItemSlots * 16 + 16 + 1024;
+  static constexpr int SMEM_BYTES = OFF_ITEMS + kItemSlots * 16 + 16;
   static_assert(SMEM_BYTES <= 232448, "shared memory of one SM");
   // TMEM columns: S_0, S_1 (P_s in the first half of S_s), O_0, O_1.
   static constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
@@ -157,6 +157,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// 4 x 4 transpose of 16-byte pieces among lanes 4k .. 4k + 3: lane r's piece c
+// goes to lane c's place r.
+__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int by) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, by), __shfl_xor_sync(0xffffffffu, v.y, by),
+                    __shfl_xor_sync(0xffffffffu, v.z, by), __shfl_xor_sync(0xffffffffu, v.w, by));
+}
+__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
+#pragma unroll
+  for (int by = 1; by <= 2; by <<= 1) {
+    const bool upper = lane & by;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & by) continue;  // exchange piece i | by of the lower lane with piece i of the upper
+      const uint4 got = shfl_xor4(upper ? w[i] : w[i | by], by);
+      if (upper) w[i] = got; else w[i | by] = got;
+    }
+  }
+}
+
 // Moves registers between the warpgroups: all warps of one execute it.
 template <int N>
 __device__ __forceinline__ void reg_inc() {
@@ -198,28 +217,6 @@ __device__ __forceinline__ float prompt_exp2(float x) {
   return y;
 }
 
-// 2^x by the polynomial units, two at a time: x = r + f, r the nearest integer
-// (the sum with 1.5 * 2^23 leaves it in the low bits), 2^f on [-1/2, 1/2] by a
-// degree-4 polynomial fitted to the least relative error (4e-6; P is rounded to
-// 2^-9 or 2^-12), r added to the exponent.  The special-function unit gives 16
-// exponentials a clock and an SM, as many clocks for a tile as its two products
-// take; a share of them done here relieves it.  x <= 8; below -126 the result
-// stays at 2^-126.
-__device__ __forceinline__ float2 poly_exp2(float2 x) {
-  constexpr float kRound = 12582912.f;
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 r = add2(x, make_float2(kRound, kRound));
-  const float2 f = fma2(add2(r, make_float2(-kRound, -kRound)), make_float2(-1.f, -1.f), x);
-  float2 y = fma2(f, make_float2(0.00957010221f, 0.00957010221f), make_float2(0.0559178591f, 0.0559178591f));
-  y = fma2(f, y, make_float2(0.240247443f, 0.240247443f));
-  y = fma2(f, y, make_float2(0.693121791f, 0.693121791f));
-  y = fma2(f, y, make_float2(0.999999285f, 0.999999285f));
-  y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23));
-  y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23));
-  return y;
-}
-
 // Rows [first, first + len) of sequence b, cut to the call's limits.
 __device__ __forceinline__ void sequence_of(const PromptParams& p, int b, int32_t& first,
                                             int32_t& len) {
@@ -232,63 +229,84 @@ __device__ __forceinline__ void sequence_of(const PromptParams& p, int b, int32_
 }
 
 
-// Item number `index` in the order of falling block number: whole warp, all
-// lanes get the result.  F(L) = items of block number >= L = sum_b max(0,
-// blocks_b - L) falls with L; the item's block is the largest L with F(L) >
-// index, and it is the (index - F(L + 1))-th sequence that has such a block.
-__device__ __forceinline__ bool find_item(const PromptParams& p, int64_t index, PromptItem& item) {
-  const int lane = static_cast<int>(threadIdx.x & 31);
-  const int32_t per = 2 * p.tq;
-  int32_t first = 0, len = 0, most = 0;
-  auto blocks = [&](int b) {
-    if (b >= p.batch) return 0;
-    sequence_of(p, b, first, len);
-    return (len + per - 1) / per;
-  };
-  const int32_t own = blocks(lane);  // of the first 32 sequences
-  auto count = [&](int32_t level) {
-    int64_t n = own > level ? own - level : 0;
-    for (int b = lane + 32; b < p.batch; b += 32) {
-      const int32_t x = blocks(b);
-      n += x > level ? x - level : 0;
+// Finds the items of the CTA, in the order of falling block number, for a whole
+// warp.  F(L) = items of block number >= L = sum_b max(0, blocks_b - L) falls
+// with L; item number `index` has as its block the largest L with F(L) > index,
+// and it is the (index - F(L + 1))-th sequence that has such a block.  32 levels
+// are tried at a time, one a lane; the first 32 sequences stay in registers.
+struct ItemFinder {
+  int32_t first, blocks, len;  // this lane's of the first 32 sequences
+  int32_t below;               // the level is below this: it falls from item to item
+  bool more;                   // more than 32 sequences
+
+  __device__ __forceinline__ void look(const PromptParams& p, int b) {
+    const int32_t per = 2 * p.tq;
+    blocks = len = first = 0;
+    if (b < p.batch) {
+      sequence_of(p, b, first, len);
+      blocks = (len + per - 1) / per;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  }
+
+  __device__ __forceinline__ void start(const PromptParams& p) {
+    below = (p.max_seqlen + 2 * p.tq - 1) / (2 * p.tq);
+    more = p.batch > 32;
+    look(p, static_cast<int>(threadIdx.x & 31));
+  }
+
+  // F at this lane's level.
+  __device__ __forceinline__ int64_t count(const PromptParams& p, int32_t level) {
+    int64_t n = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      if (more) look(p, b0 + static_cast<int>(threadIdx.x & 31));
+      int32_t part = 0;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) part += max(0, __shfl_sync(0xffffffffu, blocks, i) - level);
+      n += part;
+    }
     return n;
-  };
-  most = (p.max_seqlen + per - 1) / per;
-  int32_t level = 0, above;  // F(level) > index >= F(above)
-  if (p.batch == 1) {
-    const int32_t all = __shfl_sync(0xffffffffu, own, 0);
-    if (index >= all) return false;
-    level = all - 1 - static_cast<int32_t>(index);
-    above = level + 1;
-  } else {
-    if (count(0) <= index) return false;
-    above = most;
-    while (above - level > 1) {
-      const int32_t mid = (level + above) >> 1;
-      if (count(mid) > index) level = mid; else above = mid;
-    }
   }
-  int64_t k = index - (p.batch == 1 ? index : count(level + 1));
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const bool has = blocks(b0 + lane) > level;
-    const uint32_t mask = __ballot_sync(0xffffffffu, has);
-    if (k < __popc(mask)) {
-      int src = 0;
-      uint32_t m = mask;
-      for (; k > 0; --k) m &= m - 1;
-      src = __ffs(m) - 1;
-      item.first = __shfl_sync(0xffffffffu, first, src);
-      item.len = __shfl_sync(0xffffffffu, len, src);
-      item.t0 = level * per;
-      return true;
+
+  __device__ __forceinline__ bool find(const PromptParams& p, int64_t index, PromptItem& item) {
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    int32_t lo = 0, hi = below;  // F(lo) > index >= F(hi), if there is such an item
+    int64_t above = 0;           // F(hi)
+    bool first_round = true;
+    while (hi - lo > 1 || first_round) {
+      const int32_t step = (hi - lo + 31) / 32;
+      const int32_t level = lo + lane * step;
+      const int64_t n = count(p, min(level, hi));
+      const uint32_t yes = __ballot_sync(0xffffffffu, level < hi && n > index);
+      if (yes == 0) return false;
+      const int top = 31 - __clz(yes);
+      const int64_t next = __shfl_sync(0xffffffffu, n, min(top + 1, 31));
+      if (top < 31 && lo + (top + 1) * step < hi) {
+        above = next;
+        hi = lo + (top + 1) * step;
+      } else if (first_round) {
+        above = count(p, hi);
+      }
+      lo += top * step;
+      first_round = false;
     }
-    k -= __popc(mask);
+    below = lo + 1;
+    int64_t k = index - above;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      if (more) look(p, b0 + lane);
+      uint32_t mask = __ballot_sync(0xffffffffu, blocks > lo);
+      if (k < __popc(mask)) {
+        for (; k > 0; --k) mask &= mask - 1;
+        const int src = __ffs(mask) - 1;
+        item.first = __shfl_sync(0xffffffffu, first, src);
+        item.len = __shfl_sync(0xffffffffu, len, src);
+        item.t0 = lo * 2 * p.tq;
+        return true;
+      }
+      k -= __popc(mask);
+    }
+    return false;
   }
-  return false;
-}
+};
 
 // Row `tok` of one query head by the definition, a key at a time: whole warp.
 // Only for rows whose product with V met a NaN or an infinity at a position
@@ -343,9 +361,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                             const __grid_constant__ CUtensorMap tmap_v,
                             const __grid_constant__ PromptParams p) {
   using C = PromptCfg<DQK, DV>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // no room to align it here
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_empty = q_full + 2;
   uint64_t* k_full = q_empty + 2;
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int warp = static_cast<int>(warp_id_in_cta()), lane = static_cast<int>(threadIdx.x & 31);
   const uint64_t to = p.timeout_ns;
 
-  if (warp == 8 && lane == 0) {
+  if (warp == kLoadQK && lane == 0) {
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
@@ -387,12 +403,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     for (int i = 0; i < kItemSlots; ++i) {
       mbar_init(&i_full[i], 1);
-      mbar_init(&i_empty[i], 12);  // every warp
+      mbar_init(&i_empty[i], kPromptThreads / 32);  // every warp
     }
     *abort_flag = 0u;
     fence_mbarrier_init();
   }
-  if (warp == 9) {
+  if (warp == kMma) {
     tmem_alloc(tmem_ptr, C::TM_COLS);
     tmem_relinquish();
     tc_fence_before();
@@ -421,9 +437,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     return item.t0 + s * p.tq < item.len ? (end_of(item, s) + kKeys - 1) / kKeys : 0;
   };
 
-  if (warp >= 8) {
+  if (warp >= kLoadQK) {
     reg_dec<88>();
-    if (warp == 8) {
+    if (warp == kLoadQK) {
       // ---- loads of Q and K
       const uint32_t q_bytes = static_cast<uint32_t>(C::QH * 128 * p.group * p.tq);
       PromptItem item;
@@ -459,16 +475,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int32_t j = 1; j < n && ok; ++j) load_k(j);
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
-    } else if (warp == 11) {
+    } else if (warp == kLoadV) {
       // ---- items, two ahead of their V loads, and loads of V.  Round r takes
       // the CTA's number; odd rounds count down.
       const int32_t ctas = static_cast<int32_t>(gridDim.x), me = static_cast<int32_t>(blockIdx.x);
       bool ok = true, done = false;
+      ItemFinder finder;
+      finder.start(p);
       auto publish = [&](int32_t it) {
         if (done || !ok) return;
         const int64_t index = static_cast<int64_t>(it) * ctas + (it & 1 ? ctas - 1 - me : me);
         PromptItem item;
-        done = !find_item(p, index / p.hkv, item);
+        done = !finder.find(p, index / p.hkv, item);
         item.kvh = static_cast<int32_t>(index % p.hkv);
         if (done) item.len = 0;  // the end
         const int slot = it % kItemSlots;
@@ -495,8 +513,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               tma_load_3d(smem + C::OFF_V + vs * C::V_BYTES + h * C::HALF, &tmap_v, &v_full[vs],
                           h * 64, item.kvh, item.first + j * kKeys);
           }
-          if (j == 0) publish(it + 2);
         }
+        publish(it + 2);
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
     } else {
@@ -508,7 +526,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       // into step, both softmaxes together, then both products (18% slower).
       // A K/V tile is released by both warps; one whose row tile does not reach
       // it waits for it all the same, to count in the right phase.
-      const int s = warp - 9;
+      const int s = warp - kMma;
       const uint32_t base = smem_addr(smem);
       constexpr uint32_t kFmt = Elem16<T>::kUmmaFormat;
       constexpr uint32_t kIdescPV = make_idesc_f16(kFmt, kRows, DV) | (1u << 16);  // B along keys
@@ -550,6 +568,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           mbar_arrive(&k_empty[ks]);
         }
       };
+      // By one lane: steps [from, upto) of O += P V.
+      auto pv_steps = [&](auto from, auto upto, uint32_t steps, uint64_t vd, bool fresh) {
+        if (steps == 8u) {
+#pragma unroll
+          for (int i = decltype(from)::value; i < decltype(upto)::value; ++i)
+            umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, !fresh || i > 0);
+        } else {
+#pragma unroll 1
+          for (int i = decltype(from)::value;
+               i < min(decltype(upto)::value, static_cast<int>(steps)); ++i)
+            umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, !fresh || i > 0);
+        }
+      };
+      constexpr std::integral_constant<int, 0> kFirst{};
+      constexpr std::integral_constant<int, kMost / 16> kRest{};
+      constexpr std::integral_constant<int, kKeys / 16> kEnd{};
       auto next_k = [&]() {
         if (++ks == C::NK) {
           ks = 0;
@@ -626,19 +660,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (!ok) break;
           if (here) {
             tc_fence_after();
-            if (elect_one()) {
-              if (steps == 8u) {
-#pragma unroll
-                for (int i = 0; i < kMost / 16; ++i)
-                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV,
-                              j > 0 || i > 0);
-              } else {
-#pragma unroll 1
-                for (int i = 0; i < min(kMost / 16, static_cast<int>(steps)); ++i)
-                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV,
-                              j > 0 || i > 0);
-              }
-            }
+            if (elect_one()) pv_steps(kFirst, kRest, steps, vd, j == 0);
             __syncwarp();
             ok = mbar_wait(&p_ready[s], pp, abort_flag, to);
             pp ^= 1u;
@@ -647,15 +669,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           }
           if (elect_one()) {
             if (here) {
-              if (steps == 8u) {
-#pragma unroll
-                for (int i = kMost / 16; i < kKeys / 16; ++i)
-                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, 1u);
-              } else {
-#pragma unroll 1
-                for (int i = kMost / 16; i < static_cast<int>(steps); ++i)
-                  umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, 1u);
-              }
+              pv_steps(kRest, kEnd, steps, vd, false);
               if (last) umma_commit(&o_full[s]);
             }
             if (follows) issue_qk(j + 1 < n ? j + 1 : 0, j + 1 < n ? nt : next_nt,
@@ -686,6 +700,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int s = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    // Tokens of the warp's first and last row.
+    const int warp_tok0 = (warp & 3) * 32 / p.group, warp_tok1 = ((warp & 3) * 32 + 31) / p.group;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + lanes + C::TM_S + s * 128;
     const uint32_t tm_o = tmem + lanes + C::TM_O + s * DV;
@@ -709,39 +725,53 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tmem_ld_wait();
         float2 sum = make_float2(0.f, 0.f);
         // exp2 of 32 scores, their P and their sum.
-        auto piece = [&](auto mixed, float* v, uint32_t (&w)[16]) {
+        auto piece = [&](const float* v, uint32_t (&w)[16]) {
           const float2 scale2 = make_float2(p.qscale, p.qscale);
           const float2 shift2 = make_float2(-m_used * p.qscale, -m_used * p.qscale);
           float2 part[2];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float2 y = fma2(make_float2(v[2 * i], v[2 * i + 1]), scale2, shift2);
-            if (decltype(mixed)::value && i % kPolyEvery == kPolyEvery - 1) {
-              y = poly_exp2(y);
-            } else {
-              y.x = prompt_exp2(y.x);
-              y.y = prompt_exp2(y.y);
-            }
+            y.x = prompt_exp2(y.x);
+            y.y = prompt_exp2(y.y);
             w[i] = float2_to_pair<T>(y.x, y.y);
             part[i & 1] = i < 2 ? y : add2(part[i & 1], y);
           }
           sum = add2(sum, add2(part[0], part[1]));
         };
-        auto tile = [&](auto masked) {
-          constexpr bool kMasked = decltype(masked)::value;
-          // Masked scores must come out as zero, not as the least that the
-          // polynomial gives.
-          constexpr std::integral_constant<bool, !kMasked> mixed{};
-          if (kMasked) {
-            const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
-#pragma unroll
-            for (int i = 0; i < kKeys; ++i)
-              if (i >= seen) x[i] = -INFINITY;
+        auto store = [&](int h, const uint32_t (&w)[16]) {
+          tmem_st_32x32b_x16(tm_s + h * 16, w);
+          if (h == kMost / 32 - 1 || h == kKeys / 32 - 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h == kKeys / 32 - 1 ? &p_ready[s] : &p_most[s]);
           }
-          // The first piece goes ahead with the maximum so far, while the tile's
-          // own is found; rarely, it has to be done again.
+        };
+        // A new maximum for the rows: what was summed so far is brought to it.
+        auto move_max = [&](float m_tile) {
+          // PV(j - 1) is complete (see the order of issue) and PV(j) waits for
+          // this P, so O is this warp's to change.
+          const float m_new = fmaxf(m_used, m_tile);
+          const float c = prompt_exp2((m_used - m_new) * p.qscale);
+          m_used = m_new;
+          l *= c;
+#pragma unroll
+          for (int b = 0; b < DV; b += 16) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tm_o + b, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+            tmem_st_32x32b_x16(tm_o + b, o);
+          }
+        };
+        const int32_t least = t0 + warp_tok0 + 1 - j * kKeys;
+        if (j > 0 && least >= kKeys) {
+          // Every row sees the whole tile.  The first piece goes ahead with the
+          // maximum so far, while the tile's own is found; rarely, it has to be
+          // done again.
           uint32_t w[16];
-          if (j > 0) piece(mixed, x, w);
           float mx[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) mx[e] = fmaxf(x[e], x[4 + e]);
@@ -749,83 +779,101 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           for (int i = 8; i < kKeys; i += 8)
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + 2 * e], x[i + 2 * e + 1]);
+          piece(x, w);
           const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          const bool grow = j == 0 || (m_tile - m_used) * p.qscale > kLag;
-          if (__any_sync(0xffffffffu, grow)) {
-            if (j == 0) {
-              m_used = m_tile;
-            } else {
-              // PV(j - 1) is complete (see the order of issue) and PV(j) waits
-              // for this P, so O is this warp's to change.
-              const float m_new = fmaxf(m_used, m_tile);
-              const float c = prompt_exp2((m_used - m_new) * p.qscale);
-              m_used = m_new;
-              l *= c;
-#pragma unroll
-              for (int b = 0; b < DV; b += 16) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(tm_o + b, o);
-                tmem_ld_wait();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
-                tmem_st_32x32b_x16(tm_o + b, o);
-              }
-            }
+          if (__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag)) {
+            move_max(m_tile);
             sum = make_float2(0.f, 0.f);
-            piece(std::integral_constant<bool, false>{}, x, w);
+            piece(x, w);
           }
-          // P in pieces of 32 keys; the MMA warp starts on the first ones while
-          // the last is computed.
-          tmem_st_32x32b_x16(tm_s, w);
+          store(0, w);
 #pragma unroll
           for (int h = 1; h < kKeys / 32; ++h) {
-            piece(mixed, x + h * 32, w);
-            tmem_st_32x32b_x16(tm_s + h * 16, w);
-            if (h == kMost / 32 - 1 || h == kKeys / 32 - 1) {
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(h == kKeys / 32 - 1 ? &p_ready[s] : &p_most[s]);
-            }
+            piece(x + h * 32, w);
+            store(h, w);
           }
-          l += sum.x + sum.y;
-        };
-        if (j * kKeys + kKeys > t0 + 1)
-          tile(std::integral_constant<bool, true>{});
-        else
-          tile(std::integral_constant<bool, false>{});
+        } else {
+          // The first tile, or one that some row does not see whole.
+          const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
+          const int32_t most = t0 + warp_tok1 + 1 - j * kKeys;  // and that any row of the warp does
+          float m_tile = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < kKeys / 32; ++h) {
+            if (h * 32 >= most) continue;
+            if (least < h * 32 + 32) {
+#pragma unroll
+              for (int i = h * 32; i < h * 32 + 32; ++i)
+                if (i >= seen) x[i] = -INFINITY;
+            }
+            float m2 = m_tile;
+#pragma unroll
+            for (int i = h * 32; i < h * 32 + 32; i += 4) {
+              m_tile = max3(m_tile, x[i], x[i + 1]);
+              m2 = max3(m2, x[i + 2], x[i + 3]);
+            }
+            m_tile = fmaxf(m_tile, m2);
+          }
+          if (j == 0)
+            m_used = m_tile;
+          else if (__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag))
+            move_max(m_tile);
+#pragma unroll
+          for (int h = 0; h < kKeys / 32; ++h) {
+            uint32_t w[16];
+            if (h * 32 < most) {
+              piece(x + h * 32, w);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) w[i] = 0u;
+            }
+            store(h, w);
+          }
+        }
+        l += sum.x + sum.y;
       }
       ok = ok && mbar_wait(&o_full[s], no++ & 1u, abort_flag, to);
       if (!ok) break;
       tc_fence_after();
       const float inv = 1.f / l;
       const int head = item.kvh * p.group + row_head;
-      T* out = static_cast<T*>(p.out) + static_cast<int64_t>(item.first + tok) * p.out_token +
-               static_cast<int64_t>(head) * p.out_head;
       const bool live = row_tok < p.tq && tok < item.len;
-      bool odd = false;  // a value that is not finite
+      // Offset of the row in the output, -1: no such row.
+      const int64_t at = live ? static_cast<int64_t>(item.first + tok) * p.out_token +
+                                    static_cast<int64_t>(head) * p.out_head
+                              : -1;
+      int64_t to_row[4];  // of rows 4 (lane / 4) + i
 #pragma unroll
-      for (int b = 0; b < DV; b += 32) {
+      for (int i = 0; i < 4; ++i) to_row[i] = __shfl_sync(0xffffffffu, at, (lane & ~3) + i);
+      float2 odd = make_float2(0.f, 0.f);  // not zero if a value is not finite
+#pragma unroll
+      for (int d = 0; d < DV; d += 32) {
         uint32_t o[32];
-        tmem_ld_32x32b_x32(tm_o + b, o);
+        tmem_ld_32x32b_x32(tm_o + d, o);
         tmem_ld_wait();
-        float f[32];
+        uint4 w[4];  // the row's 32 values, 8 a piece
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          f[i] = __uint_as_float(o[i]) * inv;
-          odd |= !(fabsf(f[i]) <= FLT_MAX);
-        }
-        if (live) {
+        for (int i = 0; i < 4; ++i) {
+          uint32_t u[4];
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(out + b + i) =
-                make_uint4(float2_to_pair<T>(f[i], f[i + 1]), float2_to_pair<T>(f[i + 2], f[i + 3]),
-                           float2_to_pair<T>(f[i + 4], f[i + 5]),
-                           float2_to_pair<T>(f[i + 6], f[i + 7]));
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = make_float2(__uint_as_float(o[i * 8 + 2 * e]) * inv,
+                                         __uint_as_float(o[i * 8 + 2 * e + 1]) * inv);
+            odd = fma2(f, make_float2(0.f, 0.f), odd);
+            u[e] = float2_to_pair<T>(f.x, f.y);
+          }
+          w[i] = make_uint4(u[0], u[1], u[2], u[3]);
         }
+        // Four lanes exchange pieces, so that a store covers 64 contiguous bytes
+        // of eight rows (a row a lane would be 32 separate 16-byte pieces).
+        transpose4(w, lane);
+        T* out = static_cast<T*>(p.out) + d + (lane & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (to_row[i] >= 0) *reinterpret_cast<uint4*>(out + to_row[i]) = w[i];
       }
       tc_fence_before();
-      for (uint32_t again = __ballot_sync(0xffffffffu, odd && live); again; again &= again - 1) {
+      for (uint32_t again = __ballot_sync(0xffffffffu, live && !(odd.x + odd.y == 0.f)); again;
+           again &= again - 1) {
         const int src = __ffs(again) - 1;
         // Keys that the row's MMAs covered, up to a whole step past its tile.
         const int32_t covered = min(item.len, (end_of(item, s) + 15) / 16 * 16);
@@ -835,7 +883,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   }
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMma) {
     tc_fence_after();
     tmem_dealloc(tmem, C::TM_COLS);
   }
