@@ -14,10 +14,11 @@
 // in that order.  A short sequence thus fills its tiles G times as well, the
 // causal edge is G times finer, and every K/V tile serves two row tiles.
 // Items are numbered by falling length of their key range (the last blocks of
-// the longest sequences first), so that the device ends evenly.
+// the longest sequences first), so that the device ends evenly; KV heads whose
+// keys and values would not fit L2 together come one group after the other.
 //
-// One CTA an SM takes items in that order, counting up in one round and down in
-// the next.  Two row tiles an item take turns on the tensor core:
+// There is a CTA for each item; those that run take over the items of CTAs that
+// have not been launched, in that order.  Two row tiles an item take turns on the tensor core:
 //   S_s = Q_s K_j^T   (128 rows x 128 keys, operands in shared memory)
 //   O_s += P_s V_j    (P_s from TMEM, where it overwrites S_s; V from shared
 //                      memory as it lies, keys being the slow dimension)
@@ -51,11 +52,10 @@
 
 namespace frn {
 
-constexpr int kPromptThreads = 384;
+constexpr int kPromptThreads = 512;
 constexpr int kRows = 128;   // rows of a tile
-constexpr int kKeys = 128;   // keys of a K/V tile
-constexpr int kLoadQK = 8, kMma = 9, kLoadV = 11;  // warps; 0-3 and 4-7: softmax
-constexpr int kMost = 96;        // keys whose P is announced before the rest
+// Warps: 0-3 and 4-7 softmax of row tile 0 and 1, 8-11 output.
+constexpr int kOut = 8, kLoadQK = 12, kMma = 13, kLoadV = 15;
 constexpr int kItemSlots = 4;  // items that the scheduler is ahead
 constexpr float kLag = 8.f;  // log2 of the most that a probability may exceed 1
 
@@ -68,16 +68,27 @@ struct PromptItem {
 template <int DQK, int DV>
 struct PromptCfg {
   static constexpr int QH = DQK / 64, VH = DV / 64;  // 64-column halves (128-byte rows)
-  static constexpr int HALF = kKeys * 128;           // bytes of 128 rows x 64 columns
-  static constexpr int Q_BYTES = QH * HALF, K_BYTES = QH * HALF, V_BYTES = VH * HALF;
-  // As many K and V tiles as fit beside the two Q tiles.
-  static constexpr int NK = DQK == 192 ? 2 : DQK == 128 ? 3 : 5;
-  static constexpr int NV = DQK == 192 ? 1 : DQK == 128 ? 2 : 5;
+  // Keys of a K/V tile.  With 192 columns 96 of them, so that K and V tiles fit
+  // twice beside the two Q tiles (with 128 a second V tile does not, and every
+  // tile waits for its V; with 64 a product of 64 x 16 keys takes 48 clocks of the
+  // tensor core where 32 would do, for its operands' shared-memory reads).
+  static constexpr int KEYS = DQK == 192 ? 96 : 128;
+  static constexpr int MOST = KEYS - 32;             // keys whose P is announced before the rest
+  static constexpr int QHALF = kRows * 128;          // bytes of 128 rows x 64 columns
+  static constexpr int HALF = KEYS * 128;            // and of a K/V tile's
+  static constexpr int Q_BYTES = QH * QHALF, K_BYTES = QH * HALF, V_BYTES = VH * HALF;
+  // As many K and V tiles as fit.
+  static constexpr int NK = DQK == 64 ? 5 : 2;
+  static constexpr int NV = DQK == 64 ? 5 : 2;
+  // Staging of an output warp: pieces of 32 rows x 32 columns.
+  static constexpr int NOUT = DQK == 128 ? 4 : DQK == 192 ? 1 : 2;
   static constexpr int OFF_K = 2 * Q_BYTES;
   static constexpr int OFF_V = OFF_K + NK * K_BYTES;
-  static constexpr int OFF_BAR = OFF_V + NV * V_BYTES;
-  static constexpr int OFF_ITEMS = OFF_BAR + (12 + 2 * NK + 2 * NV + 2 * kItemSlots) * 8;
-  static constexpr int SMEM_BYTES = OFF_ITEMS + kItemSlots * 16 + 16;
+  static constexpr int OFF_OUT = OFF_V + NV * V_BYTES;
+  static constexpr int OFF_BAR = OFF_OUT + 4 * NOUT * 2048;
+  static constexpr int OFF_ITEMS = OFF_BAR + (20 + 2 * NK + 2 * NV + 2 * kItemSlots) * 8;
+  static constexpr int OFF_L = OFF_ITEMS + kItemSlots * 16 + 32;  // [parity][row tile][row] sums
+  static constexpr int SMEM_BYTES = OFF_L + 2048;
   static_assert(SMEM_BYTES <= 232448, "shared memory of one SM");
   // TMEM columns: S_0, S_1 (P_s in the first half of S_s), O_0, O_1.
   static constexpr uint32_t TM_S = 0, TM_O = 256, TM_COLS = 512;
@@ -90,7 +101,7 @@ struct PromptParams {
   void* out;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;  // elements
   const int32_t* cu;
-  int32_t batch, tokens, max_seqlen, group, hkv, tq;
+  int32_t batch, tokens, max_seqlen, group, hkv, tq, heads_at_once;
   float qscale;     // |scale| * log2(e), never zero
   uint32_t negate;  // scale < 0: S is computed with Q negated
   uint64_t timeout_ns;
@@ -141,6 +152,15 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
   asm("{\n\t.reg .b64 a, b, d;\n\t"
@@ -157,23 +177,31 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
-// 4 x 4 transpose of 16-byte pieces among lanes 4k .. 4k + 3: lane r's piece c
-// goes to lane c's place r.
-__device__ __forceinline__ uint4 shfl_xor4(uint4 v, int by) {
-  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, by), __shfl_xor_sync(0xffffffffu, v.y, by),
-                    __shfl_xor_sync(0xffffffffu, v.z, by), __shfl_xor_sync(0xffffffffu, v.w, by));
+// Asks for the number of a CTA of this grid that has not been launched yet, which
+// then never will be; the 16-byte answer completes on `bar`.
+__device__ __forceinline__ void take_cta(void* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+      " [%0], [%1];" ::"r"(smem_addr(answer)),
+      "r"(smem_addr(bar))
+      : "memory");
 }
-__device__ __forceinline__ void transpose4(uint4 (&w)[4], int lane) {
-#pragma unroll
-  for (int by = 1; by <= 2; by <<= 1) {
-    const bool upper = lane & by;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i & by) continue;  // exchange piece i | by of the lower lane with piece i of the upper
-      const uint4 got = shfl_xor4(upper ? w[i] : w[i | by], by);
-      if (upper) w[i] = got; else w[i | by] = got;
-    }
-  }
+
+// The answer: false if there was no such CTA (after which none may be asked for).
+__device__ __forceinline__ bool taken_cta(const void* answer, uint32_t& cta) {
+  uint32_t yes, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t.reg .b32 y, z, w;\n\t"
+      "mov.b32 %1, 0;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, a;\n\t}"
+      : "=&r"(yes), "=&r"(x)
+      : "r"(smem_addr(answer))
+      : "memory");
+  cta = x;
+  return yes != 0;
 }
 
 // Moves registers between the warpgroups: all warps of one execute it.
@@ -211,6 +239,23 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* m, int32_t c0, int32_t c1,
+                                                int32_t c2, int32_t c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t smem_src, int32_t c0,
+                                             int32_t c1, int32_t c2, int32_t c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::
+          "l"(reinterpret_cast<uint64_t>(m)),
+      "r"(smem_src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
 __device__ __forceinline__ float prompt_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -236,7 +281,8 @@ __device__ __forceinline__ void sequence_of(const PromptParams& p, int b, int32_
 // are tried at a time, one a lane; the first 32 sequences stay in registers.
 struct ItemFinder {
   int32_t first, blocks, len;  // this lane's of the first 32 sequences
-  int32_t below;               // the level is below this: it falls from item to item
+  int32_t below;               // the level is below this: it falls as the number grows
+  int64_t last;                // the last number looked for
   bool more;                   // more than 32 sequences
 
   __device__ __forceinline__ void look(const PromptParams& p, int b) {
@@ -248,8 +294,13 @@ struct ItemFinder {
     }
   }
 
+  __device__ __forceinline__ int32_t most(const PromptParams& p) {
+    return (p.max_seqlen + 2 * p.tq - 1) / (2 * p.tq);
+  }
+
   __device__ __forceinline__ void start(const PromptParams& p) {
-    below = (p.max_seqlen + 2 * p.tq - 1) / (2 * p.tq);
+    below = most(p);
+    last = 0;
     more = p.batch > 32;
     look(p, static_cast<int>(threadIdx.x & 31));
   }
@@ -269,6 +320,8 @@ struct ItemFinder {
 
   __device__ __forceinline__ bool find(const PromptParams& p, int64_t index, PromptItem& item) {
     const int lane = static_cast<int>(threadIdx.x & 31);
+    if (index < last) below = most(p);
+    last = index;
     int32_t lo = 0, hi = below;  // F(lo) > index >= F(hi), if there is such an item
     int64_t above = 0;           // F(hi)
     bool first_round = true;
@@ -359,8 +412,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     prompt_attention_kernel(const __grid_constant__ CUtensorMap tmap_q,
                             const __grid_constant__ CUtensorMap tmap_k,
                             const __grid_constant__ CUtensorMap tmap_v,
+                            const __grid_constant__ CUtensorMap tmap_o,
                             const __grid_constant__ PromptParams p) {
   using C = PromptCfg<DQK, DV>;
+  constexpr int kKeys = C::KEYS;
   extern __shared__ __align__(1024) uint8_t smem[];  // no room to align it here
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* q_empty = q_full + 2;
@@ -372,10 +427,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* p_ready = s_full + 2;
   uint64_t* p_most = p_ready + 2;
   uint64_t* o_full = p_most + 2;
-  uint64_t* i_full = o_full + 2;
+  uint64_t* o_empty = o_full + 2;
+  uint64_t* l_full = o_empty + 2;
+  uint64_t* i_full = l_full + 4;
   uint64_t* i_empty = i_full + kItemSlots;
+  uint64_t* answer_full = i_empty + kItemSlots;
   PromptItem* items = reinterpret_cast<PromptItem*>(smem + C::OFF_ITEMS);
-  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(items + kItemSlots);
+  uint8_t* answer = smem + C::OFF_ITEMS + kItemSlots * 16;
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(answer + 16);
   uint32_t* tmem_ptr = const_cast<uint32_t*>(abort_flag) + 1;
 
   const int warp = static_cast<int>(warp_id_in_cta()), lane = static_cast<int>(threadIdx.x & 31);
@@ -385,6 +444,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     prefetch_tmap(&tmap_q);
     prefetch_tmap(&tmap_k);
     prefetch_tmap(&tmap_v);
+    prefetch_tmap(&tmap_o);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
@@ -392,6 +452,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&p_ready[i], 4);  // the tile's softmax warps
       mbar_init(&p_most[i], 5);   // and the other tile's MMA warp, handing over
       mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 4);  // the output warps
+      mbar_init(&l_full[i], 4);  // [row tile], then the second slots
+      mbar_init(&l_full[2 + i], 4);
     }
     for (int i = 0; i < C::NK; ++i) {
       mbar_init(&k_full[i], 1);
@@ -401,6 +464,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 2);
     }
+    mbar_init(answer_full, 1);
     for (int i = 0; i < kItemSlots; ++i) {
       mbar_init(&i_full[i], 1);
       mbar_init(&i_empty[i], kPromptThreads / 32);  // every warp
@@ -438,7 +502,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   };
 
   if (warp >= kLoadQK) {
-    reg_dec<88>();
+    reg_dec<56>();
     if (warp == kLoadQK) {
       // ---- loads of Q and K
       const uint32_t q_bytes = static_cast<uint32_t>(C::QH * 128 * p.group * p.tq);
@@ -454,7 +518,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (ok && lane == 0) {
             mbar_arrive_expect_tx(&q_full[s], q_bytes);
             for (int h = 0; h < C::QH; ++h)
-              tma_load_4d(smem + s * C::Q_BYTES + h * C::HALF, &tmap_q, &q_full[s], h * 64, 0,
+              tma_load_4d(smem + s * C::Q_BYTES + h * C::QHALF, &tmap_q, &q_full[s], h * 64, 0,
                           item.kvh, item.first + item.t0 + s * p.tq);
           }
         };
@@ -469,6 +533,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                           h * 64, item.kvh, item.first + j * kKeys);
           }
         };
+        // Q waits for the last item's scores; L2 can have it already.
+        if (it > 0 && lane < 2 * C::QH) {
+          const int s = lane / C::QH;
+          if (tiles_of(item, s) > 0)
+            tma_prefetch_4d(&tmap_q, (lane % C::QH) * 64, 0, item.kvh,
+                            item.first + item.t0 + s * p.tq);
+        }
+        __syncwarp();
         load_q(0);
         load_k(0);
         load_q(1);
@@ -476,22 +548,58 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
     } else if (warp == kLoadV) {
-      // ---- items, two ahead of their V loads, and loads of V.  Round r takes
-      // the CTA's number; odd rounds count down.
-      const int32_t ctas = static_cast<int32_t>(gridDim.x), me = static_cast<int32_t>(blockIdx.x);
+      // ---- items and loads of V.  The first item is the CTA's own number; then
+      // it takes those of CTAs that have not been launched yet, each when the
+      // loads of the one before are under way: earlier, and an item would wait
+      // here while another SM is idle.
       bool ok = true, done = false;
       ItemFinder finder;
       finder.start(p);
+      const int64_t blocks = finder.count(p, 0);  // of all sequences, for one head
+      const int64_t per_group = blocks * p.heads_at_once;
+      int64_t last_group = -1;
+      uint32_t answers = 0;
+      auto ask = [&]() {
+        fence_proxy_async_smem();  // the last answer has been read
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive_expect_tx(answer_full, 16);
+          take_cta(answer, answer_full);
+        }
+      };
+      auto hear = [&](int64_t& index) {
+        ok = ok && mbar_wait(answer_full, answers++ & 1u, abort_flag, to);
+        uint32_t cta = 0;
+        const bool got = ok && taken_cta(answer, cta);
+        index = cta;
+        return got;
+      };
       auto publish = [&](int32_t it) {
         if (done || !ok) return;
-        const int64_t index = static_cast<int64_t>(it) * ctas + (it & 1 ? ctas - 1 - me : me);
+        int64_t index = blockIdx.x;
+        bool some = it == 0 || hear(index);
+        if (!ok) return;
+        const bool more = some;
+        if (more) ask();
         PromptItem item;
-        done = !finder.find(p, index / p.hkv, item);
-        item.kvh = static_cast<int32_t>(index % p.hkv);
+        if (some) {
+          const int64_t group = blocks > 0 ? index / per_group : p.hkv;
+          const int32_t head0 = static_cast<int32_t>(min(group * p.heads_at_once,
+                                                         static_cast<int64_t>(p.hkv)));
+          const int32_t heads = min(p.heads_at_once, p.hkv - head0);
+          if (group != last_group) finder.below = finder.most(p);
+          last_group = group;
+          index -= group * per_group;
+          some = heads > 0 && finder.find(p, index / heads, item);
+          item.kvh = head0 + (heads > 0 ? static_cast<int32_t>(index % heads) : 0);
+        }
+        done = !some;
         if (done) item.len = 0;  // the end
+        if (done && more)  // numbers beyond the last item: none is left to be launched
+          while (hear(index)) ask();
         const int slot = it % kItemSlots;
-        ok = mbar_wait(&i_empty[slot], (static_cast<uint32_t>(it / kItemSlots) & 1u) ^ 1u,
-                       abort_flag, to);
+        ok = ok && mbar_wait(&i_empty[slot], (static_cast<uint32_t>(it / kItemSlots) & 1u) ^ 1u,
+                             abort_flag, to);
         if (ok && lane == 0) {
           items[slot] = item;
           mbar_arrive(&i_full[slot]);
@@ -501,7 +609,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       PromptItem item;
       uint32_t nv = 0;
       publish(0);
-      publish(1);
       for (int32_t it = 0; ok && next_item(it, item); ++it) {
         const int32_t n = max(tiles_of(item, 0), tiles_of(item, 1));
         for (int32_t j = 0; j < n && ok; ++j, ++nv) {
@@ -514,7 +621,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                           h * 64, item.kvh, item.first + j * kKeys);
           }
         }
-        publish(it + 2);
+        publish(it + 1);
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
     } else {
@@ -529,6 +636,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int s = warp - kMma;
       const uint32_t base = smem_addr(smem);
       constexpr uint32_t kFmt = Elem16<T>::kUmmaFormat;
+      constexpr uint32_t kSteps = kKeys / 16;
       constexpr uint32_t kIdescPV = make_idesc_f16(kFmt, kRows, DV) | (1u << 16);  // B along keys
       const uint32_t idesc_qk = make_idesc_f16(kFmt, kRows, 0) | (p.negate << 13);
       const uint64_t qd = make_smem_desc_k_sw128(base + s * C::Q_BYTES);
@@ -536,7 +644,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const uint64_t vd0 = make_smem_desc_mn_sw128(base + C::OFF_V, C::HALF);
       const uint32_t tm_s = tmem + C::TM_S + s * 128, tm_o = tmem + C::TM_O + s * DV;
       uint32_t ks = 0, kp = 0, vs = 0, vp = 0, qp = 0, pp = 0;  // ring slots and parities
-      uint32_t mp = 0;
+      uint32_t mp = 0, op = 1;
       bool ok = true;
       // MMA steps (16 keys) of the row tile's last K/V tile.
       auto last_steps = [&](const PromptItem& x, int32_t nt) {
@@ -554,12 +662,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       auto issue_qk = [&](int32_t j, int32_t nt, uint32_t ragged) {
         if (j < nt) {
           const bool last = j + 1 == nt;
-          const uint32_t idesc = idesc_qk | ((last ? ragged : 8u) << 18);  // N = 16 a step
+          const uint32_t idesc = idesc_qk | ((last ? ragged : kSteps) << 18);  // N = 16 a step
           const uint64_t kd = kd0 + ks * (C::K_BYTES >> 4);
 #pragma unroll
           for (int i = 0; i < DQK / 16; ++i) {
-            const uint32_t off = ((i / 4) * C::HALF + (i % 4) * 32) >> 4;
-            umma_f16_ss(tm_s, qd + off, kd + off, idesc, i > 0);
+            umma_f16_ss(tm_s, qd + (((i / 4) * C::QHALF + (i % 4) * 32) >> 4),
+                        kd + (((i / 4) * C::HALF + (i % 4) * 32) >> 4), idesc, i > 0);
           }
           umma_commit(&s_full[s]);
           umma_commit(&k_empty[ks]);
@@ -570,7 +678,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       };
       // By one lane: steps [from, upto) of O += P V.
       auto pv_steps = [&](auto from, auto upto, uint32_t steps, uint64_t vd, bool fresh) {
-        if (steps == 8u) {
+        if (steps == kSteps) {
 #pragma unroll
           for (int i = decltype(from)::value; i < decltype(upto)::value; ++i)
             umma_f16_ts(tm_o, tm_s + i * 8, vd + ((i * 2048) >> 4), kIdescPV, !fresh || i > 0);
@@ -582,7 +690,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       };
       constexpr std::integral_constant<int, 0> kFirst{};
-      constexpr std::integral_constant<int, kMost / 16> kRest{};
+      constexpr std::integral_constant<int, C::MOST / 16> kRest{};
       constexpr std::integral_constant<int, kKeys / 16> kEnd{};
       auto next_k = [&]() {
         if (++ks == C::NK) {
@@ -635,9 +743,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
           }
           ok = ok && mbar_wait(&v_full[vs], vp, abort_flag, to);
+          if (j == 0 && nt > 0) {  // the last item's output is out of TMEM
+            ok = ok && mbar_wait(&o_empty[s], op, abort_flag, to);
+            op ^= 1u;
+          }
           if (!ok) break;
           const bool here = j < nt, last = j + 1 == nt;
-          const uint32_t steps = last ? ragged : 8u;
+          const uint32_t steps = last ? ragged : kSteps;
           const uint64_t vd = vd0 + vs * (C::V_BYTES >> 4);
           if (here) {
             const int32_t left = item.len - j * kKeys;
@@ -694,18 +806,125 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ragged = next_ragged;
       }
     }
+  } else if (warp >= kOut) {
+    reg_dec<104>();
+    // ---- output: O over the row's sum, while the softmax warps go on with the
+    // next item
+    const int row = (warp & 3) * 32 + lane;
+    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int warp_tok0 = (warp & 3) * 32 / p.group;  // token of the warp's first row
+    const uint32_t stage = smem_addr(smem + C::OFF_OUT) + (warp & 3) * (C::NOUT * 2048);
+    uint32_t no[2] = {0, 0};  // items so far
+    bool ok = true;
+    PromptItem item;
+    for (int32_t it = 0; ok && next_item(it, item); ++it) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (tiles_of(item, s) == 0) continue;
+        const int32_t tok = item.t0 + s * p.tq + row_tok;
+        const uint32_t tm_o = tmem + lanes + C::TM_O + s * DV;
+        const uint32_t slot = no[s] & 1u;
+        ok = ok && mbar_wait(&l_full[slot * 2 + s], (no[s] >> 1) & 1u, abort_flag, to) &&
+             mbar_wait(&o_full[s], no[s] & 1u, abort_flag, to);
+        ++no[s];
+        if (!ok) break;
+        tc_fence_after();
+        const float inv =
+            1.f / reinterpret_cast<float*>(smem + C::OFF_L)[slot * 256 + s * 128 + row];
+        const int head = item.kvh * p.group + row_head;
+        const bool live = row_tok < p.tq && tok < item.len;
+        // A warp whose rows are whole tokens, all of them there, leaves the
+        // store to TMA; else the rows go one by one.
+        const int32_t tok0 = item.t0 + s * p.tq + warp_tok0;
+        const bool bulk = 32 % p.group == 0 && tok0 + 32 / p.group <= item.len;
+        // Offset of the row in the output, -1: no such row.
+        const int64_t at = live ? static_cast<int64_t>(item.first + tok) * p.out_token +
+                                      static_cast<int64_t>(head) * p.out_head
+                                : -1;
+        float2 odd = make_float2(0.f, 0.f);  // not zero if a value is not finite
+        // TMEM first, so that the next item's products can begin.
+        uint32_t w[DV / 2];
+#pragma unroll
+        for (int d = 0; d < DV / 32; ++d) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tm_o + d * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = mul2(make_float2(__uint_as_float(o[2 * i]),
+                                              __uint_as_float(o[2 * i + 1])),
+                                  make_float2(inv, inv));
+            odd = fma2(f, make_float2(0.f, 0.f), odd);
+            w[d * 16 + i] = float2_to_pair<T>(f.x, f.y);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_empty[s]);
+#pragma unroll
+        for (int d0 = 0; d0 < DV / 32; d0 += C::NOUT) {
+          if (lane == 0) bulk_wait_group_read<0>();  // the last stores have read the staging
+          __syncwarp();
+#pragma unroll
+          for (int d = d0; d < d0 + C::NOUT; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)  // rows of 64 bytes, 64-byte swizzle
+              st_shared_v4(stage + (d - d0) * 2048 + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4),
+                           w[d * 16 + i * 4], w[d * 16 + i * 4 + 1], w[d * 16 + i * 4 + 2],
+                           w[d * 16 + i * 4 + 3]);
+          if (bulk) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+#pragma unroll
+              for (int d = d0; d < d0 + C::NOUT; ++d)
+                tma_store_4d(&tmap_o, stage + (d - d0) * 2048, d * 32, 0, item.kvh,
+                             item.first + tok0);
+              bulk_commit_group();
+            }
+          } else {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // 8 rows, 64 contiguous bytes of each piece
+              const int r = i * 8 + (lane >> 2), c = lane & 3;
+              const int64_t to_row = __shfl_sync(0xffffffffu, at, r);
+              if (to_row >= 0)
+#pragma unroll
+                for (int d = d0; d < d0 + C::NOUT; ++d)
+                  *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + to_row + d * 32 + c * 8) =
+                      ld_shared_v4(stage + (d - d0) * 2048 + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+            }
+            __syncwarp();
+          }
+        }
+        uint32_t again = __ballot_sync(0xffffffffu, live && !(odd.x + odd.y == 0.f));
+        if (again) {  // these rows are written once more, after the stores above
+          if (lane == 0) bulk_wait_group_all();
+          __syncwarp();
+        }
+        for (; again; again &= again - 1) {
+          const int src = __ffs(again) - 1;
+          // Keys that the row's MMAs covered, up to a whole step past its tile.
+          const int32_t covered = min(item.len, (end_of(item, s) + 15) / 16 * 16);
+          exact_row<T, DQK, DV>(p, item.first, __shfl_sync(0xffffffffu, tok, src), item.kvh,
+                                __shfl_sync(0xffffffffu, head, src), covered);
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group_read<0>();  // the staging is read before the CTA ends
   } else {
-    reg_inc<208>();
+    reg_inc<176>();
     // ---- softmax: one row a thread
     const int s = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
-    const int row_tok = row / p.group, row_head = row - row_tok * p.group;
+    const int row_tok = row / p.group;
     // Tokens of the warp's first and last row.
     const int warp_tok0 = (warp & 3) * 32 / p.group, warp_tok1 = ((warp & 3) * 32 + 31) / p.group;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tm_s = tmem + lanes + C::TM_S + s * 128;
     const uint32_t tm_o = tmem + lanes + C::TM_O + s * DV;
-    uint32_t ns = 0, no = 0;  // waits so far on s_full and o_full
+    uint32_t ns = 0, no = 0;  // tiles and items so far
     bool ok = true;
     PromptItem item;
     for (int32_t it = 0; ok && next_item(it, item); ++it) {
@@ -741,7 +960,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         };
         auto store = [&](int h, const uint32_t (&w)[16]) {
           tmem_st_32x32b_x16(tm_s + h * 16, w);
-          if (h == kMost / 32 - 1 || h == kKeys / 32 - 1) {
+          if (h == C::MOST / 32 - 1 || h == kKeys / 32 - 1) {
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -831,55 +1050,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
         l += sum.x + sum.y;
       }
-      ok = ok && mbar_wait(&o_full[s], no++ & 1u, abort_flag, to);
+      // The sums go to the output warps, by two slots (and barriers) in turn: the
+      // first product of the next item waits for the output of this one, so the
+      // item after next cannot be here before.
       if (!ok) break;
-      tc_fence_after();
-      const float inv = 1.f / l;
-      const int head = item.kvh * p.group + row_head;
-      const bool live = row_tok < p.tq && tok < item.len;
-      // Offset of the row in the output, -1: no such row.
-      const int64_t at = live ? static_cast<int64_t>(item.first + tok) * p.out_token +
-                                    static_cast<int64_t>(head) * p.out_head
-                              : -1;
-      int64_t to_row[4];  // of rows 4 (lane / 4) + i
-#pragma unroll
-      for (int i = 0; i < 4; ++i) to_row[i] = __shfl_sync(0xffffffffu, at, (lane & ~3) + i);
-      float2 odd = make_float2(0.f, 0.f);  // not zero if a value is not finite
-#pragma unroll
-      for (int d = 0; d < DV; d += 32) {
-        uint32_t o[32];
-        tmem_ld_32x32b_x32(tm_o + d, o);
-        tmem_ld_wait();
-        uint4 w[4];  // the row's 32 values, 8 a piece
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t u[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = make_float2(__uint_as_float(o[i * 8 + 2 * e]) * inv,
-                                         __uint_as_float(o[i * 8 + 2 * e + 1]) * inv);
-            odd = fma2(f, make_float2(0.f, 0.f), odd);
-            u[e] = float2_to_pair<T>(f.x, f.y);
-          }
-          w[i] = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-        // Four lanes exchange pieces, so that a store covers 64 contiguous bytes
-        // of eight rows (a row a lane would be 32 separate 16-byte pieces).
-        transpose4(w, lane);
-        T* out = static_cast<T*>(p.out) + d + (lane & 3) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (to_row[i] >= 0) *reinterpret_cast<uint4*>(out + to_row[i]) = w[i];
-      }
-      tc_fence_before();
-      for (uint32_t again = __ballot_sync(0xffffffffu, live && !(odd.x + odd.y == 0.f)); again;
-           again &= again - 1) {
-        const int src = __ffs(again) - 1;
-        // Keys that the row's MMAs covered, up to a whole step past its tile.
-        const int32_t covered = min(item.len, (end_of(item, s) + 15) / 16 * 16);
-        exact_row<T, DQK, DV>(p, item.first, __shfl_sync(0xffffffffu, tok, src), item.kvh,
-                              __shfl_sync(0xffffffffu, head, src), covered);
-      }
+      reinterpret_cast<float*>(smem + C::OFF_L)[(no & 1u) * 256 + s * 128 + row] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&l_full[(no & 1u) * 2 + s]);
+      ++no;
     }
   }
   __syncthreads();
@@ -906,7 +1084,7 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
   }
   const int64_t G = g.Hq / g.Hkv, tq = kRows / G;
   const CUtensorMapDataType dt = Elem16<T>::kTmaType;
-  CUtensorMap tq_map, tk, tv;
+  CUtensorMap tq_map, tk, tv, to;
   {  // (d, head of the group, KV head, token)
     const uint64_t dims[4] = {static_cast<uint64_t>(DQK), static_cast<uint64_t>(G),
                               static_cast<uint64_t>(g.Hkv), static_cast<uint64_t>(g.tokens)};
@@ -917,7 +1095,18 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
     const int rc = encode_tmap_4d(&tq_map, dt, g.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
-  const uint32_t box[3] = {64, 1, kKeys};
+  {  // the same view of the output; used where a warp's 32 rows are whole tokens
+    const uint64_t dims[4] = {static_cast<uint64_t>(DV), static_cast<uint64_t>(G),
+                              static_cast<uint64_t>(g.Hkv), static_cast<uint64_t>(g.tokens)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(g.out_head_stride) * 2,
+                                 static_cast<uint64_t>(G * g.out_head_stride) * 2,
+                                 static_cast<uint64_t>(g.out_token_stride) * 2};
+    const uint32_t box[4] = {32, static_cast<uint32_t>(32 % G == 0 ? G : 1), 1,
+                             static_cast<uint32_t>(32 % G == 0 ? 32 / G : 1)};
+    const int rc = encode_tmap_4d(&to, dt, g.out, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc) return rc;
+  }
+  const uint32_t box[3] = {64, 1, C::KEYS};
   {
     const uint64_t dims[3] = {static_cast<uint64_t>(DQK), static_cast<uint64_t>(g.Hkv),
                               static_cast<uint64_t>(g.tokens)};
@@ -954,6 +1143,13 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
   p.group = static_cast<int32_t>(G);
   p.hkv = static_cast<int32_t>(g.Hkv);
   p.tq = static_cast<int32_t>(tq);
+  // All blocks of some KV heads come before those of the next, so that the keys
+  // and values that the blocks share stay in L2 (a third of it).
+  const int64_t head_bytes = g.tokens * (DQK + DV) * 2;
+  int64_t at_once = (int64_t(40) << 20) / head_bytes;
+  if (at_once < 1) at_once = 1;
+  const int64_t groups = (g.Hkv + at_once - 1) / at_once;
+  p.heads_at_once = static_cast<int32_t>((g.Hkv + groups - 1) / groups);
   p.negate = g.scale < 0.f ? 1u : 0u;
   // A scale of zero (every key the same weight) still has to send the masked
   // scores, -inf, to -inf: any factor far below the scores' rounding will do.
@@ -967,8 +1163,9 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
   const int64_t longest = g.batch * ((g.max_seqlen + per - 1) / per);
   if (longest < items) items = longest;
   cudaLaunchConfig_t cfg = {};
-  const int64_t ctas = items * g.Hkv < sm_count(dev) ? items * g.Hkv : sm_count(dev);
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+  if (items * g.Hkv > 0x7fffffffLL)
+    return set_error(FRN_ERR_UNSUPPORTED, "prompt attention: too many work items");
+  cfg.gridDim = dim3(static_cast<unsigned>(items * g.Hkv));
   cfg.blockDim = dim3(kPromptThreads);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
@@ -977,7 +1174,7 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tq_map, tk, tv, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tq_map, tk, tv, to, p);
   if (e != cudaSuccess) return set_cuda_error("launch prompt_attention", e);
   return 0;
 }
