@@ -9,20 +9,24 @@
 // Hkv * D elements, each read once for all G query heads of its KV head.
 //
 // Split.  The lengths live on the device and differ, so the work is cut there:
-// the 64-token tiles of all (sequence, KV head) items, laid end to end, are
-// dealt to the CTAs in equal contiguous shares, whatever the lengths.  A CTA
+// the 16-token tiles of all (sequence, KV head) items, laid end to end, are
+// dealt to the warps in equal contiguous shares, whatever the lengths (an item
+// counts as at least `least` tiles, which pays for its queries and its end, and
+// keeps tiny items from sharing a warp while others idle).  A warp
 // walks its share item by item; an item that lies within one share is written
 // directly, of the others every share leaves (max, sum, acc) in the workspace
-// (at most two parts a CTA: an item can be cut at its share's start and at
+// (at most two parts a warp: an item can be cut at its share's start and at
 // its end), and a second, dependent launch joins the parts in share order.  No
-// atomics: the result does not depend on the order in which CTAs finish.
+// atomics: the result does not depend on the order in which warps finish.
+// Shares are a warp's, not a CTA's: with four warps on every tile the join of
+// the warps at each item's end cost 2 us, and a batch of 64 sequences of 1 to
+// 8192 tokens took 76 us instead of ... us.
 //
-// Streams.  The four warps of a CTA take 16 tokens of every tile each and
-// share nothing until an item ends: a warp copies its own tokens with 16-byte
-// cp.async into its own ring, several tiles ahead and across item borders, so
-// no block barrier and no page boundary interrupts the stream.  Tokens past
-// the length are never read (their slots are zero-filled and their scores are
-// -inf), so whatever lies in unused slots or pages has no effect.
+// Streams.  A warp copies its tiles with 16-byte cp.async into its own ring,
+// several tiles ahead and across item borders: no block barrier and no page
+// boundary interrupts the stream.  Tokens past the length are never read
+// (their slots are zero-filled and their scores are -inf), so whatever lies in
+// unused slots or pages has no effect.
 //
 // Arithmetic.  bf16 / fp16: the query heads of a group are the rows of 16x8x16
 // MMAs (S = Q K^T, O += P V; up to 16 heads), online softmax in base 2 on the
@@ -43,8 +47,9 @@ namespace frn {
 
 constexpr int kPagedWarps = 4;
 constexpr int kPagedThreads = 32 * kPagedWarps;
-constexpr int kWarpTokens = 16;                         // a warp's tokens of a tile
-constexpr int kTileTokens = kPagedWarps * kWarpTokens;  // 64
+constexpr int kTileTokens = 16;
+
+constexpr int paged_ctas_per_sm(bool fp32, int d) { return fp32 && d == 128 ? 1 : d == 128 ? 2 : fp32 ? 2 : 4; }
 
 struct PagedDecodeParams {
   PagedView kv;
@@ -53,26 +58,25 @@ struct PagedDecodeParams {
   void* out;
   int64_t out_batch, out_head;  // element strides
   const int32_t* seq_lens;
-  float* ws;       // [2 * CTAs][G][D] accumulators, then [2 * CTAs][G][2] (max, sum)
-  int32_t* joins;  // [batch * Hkv][2] first part's slot (-1: nothing to join), last CTA
-  int32_t batch, hkv, group, ctas;
+  float* ws;       // [2 * warps][G][D] accumulators, then [2 * warps][G][2] (max, sum)
+  int32_t* joins;  // [batch * Hkv][2] first part (-1: nothing to join), last warp
+  int32_t batch, hkv, group, warps, least;
   float qscale;    // scale * log2(e): the softmax runs in base 2
 };
 
 template <typename T, int D, int GMAX>
 struct PagedCfg {
   static constexpr int ROW_BYTES = D * static_cast<int>(sizeof(T));
-  static constexpr int HALF_BYTES = kWarpTokens * ROW_BYTES;  // a warp's K (or V) of a tile
+  static constexpr int HALF_BYTES = kTileTokens * ROW_BYTES;  // K (or V) of a tile
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
-  // 24 KB of ring a warp, two CTAs an SM; the 512-byte rows of fp32 at D = 128
-  // take 48 KB and an SM each.
-  static constexpr int CTAS_PER_SM = HALF_BYTES > 4096 ? 1 : 2;
-  static constexpr int STAGES = (CTAS_PER_SM == 1 ? 49152 : 24576) / STAGE_BYTES;
-  static constexpr int RING_BYTES = kPagedWarps * STAGES * STAGE_BYTES;
-  // Join of the four warps: 8 heads at a time, [warp][8][D] acc, [warp][8] max and sum.
-  static constexpr int JOIN_FLOATS = kPagedWarps * 8 * (D + 2);
-  static constexpr int Q_FLOATS = sizeof(T) == 4 ? GMAX * D : 0;  // fp32: the queries
-  static constexpr int SMEM_BYTES = RING_BYTES + (JOIN_FLOATS + Q_FLOATS) * 4;
+  // CTAs an SM: as many warps as their rings leave room for.
+  static constexpr int CTAS_PER_SM = paged_ctas_per_sm(sizeof(T) == 4, D);
+  static constexpr int STAGES = (224 * 1024 / CTAS_PER_SM / kPagedWarps - (sizeof(T) == 4 ? GMAX * D * 4 : 0)) / STAGE_BYTES;
+  static constexpr int RING_BYTES = STAGES * STAGE_BYTES;
+  static constexpr int Q_BYTES = sizeof(T) == 4 ? GMAX * D * 4 : 0;  // fp32: the item's queries
+  static constexpr int WARP_BYTES = RING_BYTES + Q_BYTES;
+  static constexpr int SMEM_BYTES = kPagedWarps * WARP_BYTES;
+  static_assert(STAGES >= 2, "one tile in flight while one is used");
 };
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -126,9 +130,11 @@ __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
                  : "memory");
 }
 
-// A place in the sequence of tiles: tile `tile` of the item (b, head).
+// A place in the sequence of tiles: tile `tile` of the item (b, head), at
+// position u of all.
 struct TileAt {
   int32_t b, head, tile, tiles, len;
+  int64_t u;
 };
 
 // Length of sequence b as the kernel uses it: not negative, and within the
@@ -147,13 +153,21 @@ __device__ __forceinline__ int32_t tiles_of(int32_t len) {
   return static_cast<int32_t>((static_cast<int64_t>(len) + kTileTokens - 1) / kTileTokens);
 }
 
+// Positions that an item of a sequence takes up.
+__device__ __forceinline__ int32_t places_of(const PagedDecodeParams& p, int32_t tiles) {
+  return tiles > 0 ? max(tiles, p.least) : 0;
+}
+
+// The next tile; past the last one u is the total.
 __device__ __forceinline__ void advance(const PagedDecodeParams& p, TileAt& at) {
+  ++at.u;
   if (++at.tile < at.tiles) return;
+  at.u += places_of(p, at.tiles) - at.tiles;
   at.tile = 0;
   if (++at.head < p.hkv) return;
   at.head = 0;
   do {
-    if (++at.b >= p.batch) return;  // past the last tile: not used any more
+    if (++at.b >= p.batch) return;
     at.len = length_of(p, at.b);
     at.tiles = tiles_of(at.len);
   } while (at.tiles == 0);
@@ -178,7 +192,7 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// Tiles before sequence b, times Hkv, for every b at once: thread i sums its
+// Positions before sequence b, for every b at once: thread i sums its
 // run of sequences, a block scan does the rest.  Returns the total; *mine is
 // the sum of the runs before this thread's.
 __device__ __forceinline__ int64_t scan_tiles(const PagedDecodeParams& p, int64_t* sm_warp,
@@ -186,7 +200,7 @@ __device__ __forceinline__ int64_t scan_tiles(const PagedDecodeParams& p, int64_
   const int per = (p.batch + kPagedThreads - 1) / kPagedThreads;
   const int b0 = static_cast<int>(threadIdx.x) * per;
   int64_t sum = 0;
-  for (int b = b0; b < min(p.batch, b0 + per); ++b) sum += tiles_of(length_of(p, b));
+  for (int b = b0; b < min(p.batch, b0 + per); ++b) sum += places_of(p, tiles_of(length_of(p, b)));
   sum *= p.hkv;
   const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
   int64_t inc = sum;
@@ -208,8 +222,9 @@ __device__ __forceinline__ int64_t scan_tiles(const PagedDecodeParams& p, int64_
   return total;
 }
 
-template <typename T, int D, int GMAX>
-__global__ void __launch_bounds__(kPagedThreads, 2)
+// UNI: pages hold whole tiles, so a tile's rows are `token_stride` apart.
+template <typename T, int D, int GMAX, bool UNI>
+__global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 4, D))
     paged_decode_kernel(const PagedDecodeParams p) {
   using C = PagedCfg<T, D, GMAX>;
   constexpr bool MMA = sizeof(T) == 2;
@@ -219,52 +234,64 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
   constexpr int CHUNKS = C::ROW_BYTES / 16;     // 16-byte pieces of a row
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t sm_warp[kPagedWarps];
-  __shared__ TileAt sm_first;
+  __shared__ TileAt sm_first[kPagedWarps];
 
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const int G = p.group;
   griddep_launch_dependents();
   griddep_wait();
 
-  // ---- this CTA's share [u0, u1) of the tiles, and where it starts
+  // ---- the warps' shares of the tiles, and where they start
   int64_t before, own;
   const int64_t total = scan_tiles(p, sm_warp, &before, &own);
-  const int64_t share = (total + p.ctas - 1) / p.ctas;
-  const int64_t u0 = share * blockIdx.x, u1 = min(total, u0 + share);
-  if (u0 >= u1) return;
-  if (before <= u0 && u0 < before + own) {  // one thread's run holds tile u0
+  const int64_t share = max((total + p.warps - 1) / p.warps, static_cast<int64_t>(p.least));
+  const int me = static_cast<int>(blockIdx.x) * kPagedWarps + warp;  // this warp's number
+  if (own > 0) {
+    // The shares of this CTA that start within this thread's run of sequences.
     const int per = (p.batch + kPagedThreads - 1) / kPagedThreads;
-    int b = static_cast<int>(threadIdx.x) * per;
-    int64_t at = before;
-    TileAt f;
-    for (;; ++b) {
-      f.len = length_of(p, b);
-      f.tiles = tiles_of(f.len);
-      const int64_t n = static_cast<int64_t>(f.tiles) * p.hkv;
-      if (u0 < at + n) break;
-      at += n;
+    for (int w = 0; w < kPagedWarps; ++w) {
+      const int64_t u = share * (static_cast<int64_t>(blockIdx.x) * kPagedWarps + w);
+      if (u < before || u >= before + own) continue;
+      int b = static_cast<int>(threadIdx.x) * per;
+      int64_t at = before;
+      TileAt f;
+      for (;; ++b) {
+        f.len = length_of(p, b);
+        f.tiles = tiles_of(f.len);
+        const int64_t n = static_cast<int64_t>(places_of(p, f.tiles)) * p.hkv;
+        if (u < at + n) break;
+        at += n;
+      }
+      const int32_t places = places_of(p, f.tiles);
+      f.b = b;
+      f.head = static_cast<int32_t>((u - at) / places);
+      f.tile = static_cast<int32_t>((u - at) % places);
+      f.u = u;
+      if (f.tile >= f.tiles) {  // past the item's tiles: the next item
+        f.u -= f.tile - (f.tiles - 1);
+        f.tile = f.tiles - 1;
+        advance(p, f);
+      }
+      sm_first[w] = f;
     }
-    f.b = b;
-    f.head = static_cast<int32_t>((u0 - at) / f.tiles);
-    f.tile = static_cast<int32_t>((u0 - at) % f.tiles);
-    sm_first = f;
   }
   __syncthreads();
-  TileAt now = sm_first, ahead = now;
-  const int64_t ntiles = u1 - u0;
+  const int64_t u0 = share * me, u1 = min(total, u0 + share);
+  if (u0 >= u1) return;
+  TileAt now = sm_first[warp], ahead = now;
+  if (now.u >= u1) return;
 
-  uint8_t* ring = smem + warp * (C::STAGES * C::STAGE_BYTES);
+  uint8_t* ring = smem + warp * C::WARP_BYTES;
   const uint32_t ring_a = smem_addr(ring);
-  float* sm_acc = reinterpret_cast<float*>(smem + C::RING_BYTES);  // [4][8][D]
-  float* sm_m = sm_acc + kPagedWarps * 8 * D;                      // [4][8]
-  float* sm_l = sm_m + kPagedWarps * 8;                            // [4][8]
-  float* sm_q = sm_acc + C::JOIN_FLOATS;                           // fp32: [G][D]
+  float* sm_q = reinterpret_cast<float*>(ring + C::RING_BYTES);  // fp32: [G][D]
 
-  // ---- loads: lane r < 16 looks up the page of the warp's token r one tile
-  // before that tile's copies are issued.
+  // ---- loads: the page of a tile (or of each of its tokens, one a lane) is
+  // looked up one tile before the tile's copies are issued.
+  constexpr int ROWS = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;  // rows of one pass of the warp
+  const int my_row = lane / CHUNKS, my_col = lane % CHUNKS;
   int32_t page = -1, slot = 0;
   auto look_up = [&]() {
-    const int32_t t = ahead.tile * kTileTokens + warp * kWarpTokens + (lane & 15);
+    const int32_t t = ahead.tile * kTileTokens + (UNI ? 0 : (lane & 15));
     page = -1;
     if (t < ahead.len) {
       const int32_t n = t / p.kv.page_size;
@@ -278,37 +305,54 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
   };
   auto issue = [&](int stage) {
     const uint32_t kdst = ring_a + stage * C::STAGE_BYTES, vdst = kdst + C::HALF_BYTES;
-    constexpr int ROWS = 32 / CHUNKS > 0 ? 32 / CHUNKS : 1;  // rows of one pass of the warp
-    const T* kb = static_cast<const T*>(p.kv.k) + ahead.head * p.kv.k_head_stride;
-    const T* vb = static_cast<const T*>(p.kv.v) + ahead.head * p.kv.v_head_stride;
-    const int c = lane % CHUNKS;
+    const T* kb = static_cast<const T*>(p.kv.k) + ahead.head * p.kv.k_head_stride +
+                  my_col * (16 / sizeof(T));
+    const T* vb = static_cast<const T*>(p.kv.v) + ahead.head * p.kv.v_head_stride +
+                  my_col * (16 / sizeof(T));
+    const int64_t kt = p.kv.k_token_stride, vt = p.kv.v_token_stride;
+    const int32_t left = ahead.len - ahead.tile * kTileTokens;
+    if constexpr (UNI) {
+      const int64_t pp = page >= 0 ? page : 0;
+      const int32_t rows = page >= 0 ? left : 0;
+      kb += pp * p.kv.k_page_stride + (slot + my_row) * kt;
+      vb += pp * p.kv.v_page_stride + (slot + my_row) * vt;
 #pragma unroll
-    for (int i = 0; i < kWarpTokens / ROWS; ++i) {
-      const int r = i * ROWS + lane / CHUNKS;
-      const int32_t pg = __shfl_sync(0xffffffffu, page, r);
-      const int64_t sl = __shfl_sync(0xffffffffu, slot, r);
-      const uint32_t bytes = pg >= 0 ? 16u : 0u;
-      const int64_t pp = pg >= 0 ? pg : 0;
-      const T* ks = kb + pp * p.kv.k_page_stride + sl * p.kv.k_token_stride + c * (16 / sizeof(T));
-      const T* vs = vb + pp * p.kv.v_page_stride + sl * p.kv.v_token_stride + c * (16 / sizeof(T));
-      cp_async_16(kdst + swz<C::ROW_BYTES>(r, c), ks, bytes);
-      cp_async_16(vdst + swz<C::ROW_BYTES>(r, c), vs, bytes);
-    }
-  };
-  int64_t issued = 0;
-  look_up();
+      for (int i = 0; i < kTileTokens / ROWS; ++i) {
+        const int r = i * ROWS + my_row;
+        const uint32_t bytes = r < rows ? 16u : 0u;
+        cp_async_16(kdst + swz<C::ROW_BYTES>(r, my_col), kb, bytes);
+        cp_async_16(vdst + swz<C::ROW_BYTES>(r, my_col), vb, bytes);
+        if (r + ROWS < rows) {  // a row that is not read keeps an address that is
+          kb += ROWS * kt;
+          vb += ROWS * vt;
+        }
+      }
+    } else {
 #pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s) {
-    if (issued < ntiles) {
-      issue(s);
-      ++issued;
-      if (issued < ntiles) {
-        advance(p, ahead);
-        look_up();
+      for (int i = 0; i < kTileTokens / ROWS; ++i) {
+        const int r = i * ROWS + my_row;
+        const int32_t pg = __shfl_sync(0xffffffffu, page, r);
+        const int64_t sl = __shfl_sync(0xffffffffu, slot, r);
+        const uint32_t bytes = pg >= 0 ? 16u : 0u;
+        const int64_t pp = pg >= 0 ? pg : 0;
+        cp_async_16(kdst + swz<C::ROW_BYTES>(r, my_col),
+                    kb + pp * p.kv.k_page_stride + (pg >= 0 ? sl * kt : 0), bytes);
+        cp_async_16(vdst + swz<C::ROW_BYTES>(r, my_col),
+                    vb + pp * p.kv.v_page_stride + (pg >= 0 ? sl * vt : 0), bytes);
       }
     }
+  };
+  auto issue_next = [&](int stage) {
+    if (ahead.u < u1) {
+      issue(stage);
+      advance(p, ahead);
+      if (ahead.u < u1) look_up();
+    }
     cp_async_commit();
-  }
+  };
+  look_up();
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) issue_next(s);
 
   // ---- per item: queries, running statistics, accumulators
   const int g = lane >> 2, tq = lane & 3;
@@ -321,19 +365,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
   bool first_segment = true;
   int stage = 0;
 
-  for (int64_t u = 0; u < ntiles; ++u) {
+  while (now.u < u1) {
     // Keep the ring full: the slot freed by the previous tile takes a new one.
-    if (issued < ntiles) {
-      int s = stage + C::STAGES - 1;
-      if (s >= C::STAGES) s -= C::STAGES;
-      issue(s);
-      ++issued;
-      if (issued < ntiles) {
-        advance(p, ahead);
-        look_up();
-      }
-    }
-    cp_async_commit();
+    issue_next(stage == 0 ? C::STAGES - 1 : stage - 1);
 
     if (fresh) {
       fresh = false;
@@ -357,10 +391,10 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
           l_run[r] = 0.f;
         }
       } else {
-        __syncthreads();  // every warp is done with the last item's queries
-        for (int i = static_cast<int>(threadIdx.x); i < G * D; i += kPagedThreads)
+        __syncwarp();  // every lane is done with the last item's queries
+        for (int i = lane; i < G * D; i += 32)
           sm_q[i] = static_cast<float>(qp[(i / D) * p.q_head + i % D]);
-        __syncthreads();
+        __syncwarp();
 #pragma unroll
         for (int r = 0; r < GMAX; ++r) {
           m_run[r] = -FLT_MAX;
@@ -374,9 +408,9 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
     cp_async_wait<C::STAGES - 1>();
     __syncwarp();
     const uint32_t kb = ring_a + stage * C::STAGE_BYTES, vb = kb + C::HALF_BYTES;
-    const int32_t t0 = now.tile * kTileTokens + warp * kWarpTokens;  // the warp's first token
+    const int32_t left = now.len - now.tile * kTileTokens;  // tokens from the tile's first on
     if constexpr (MMA) {
-      // S = Q . K^T of this warp's 16 tokens: two 8-token tiles.
+      // S = Q . K^T of the 16 tokens: two 8-token tiles.
       float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int kc = 0; kc < NKC; ++kc) {
@@ -391,23 +425,26 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
         float x[4];  // columns: tokens 2tq, 2tq + 1 of each tile
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int32_t t = t0 + (e >> 1) * 8 + 2 * tq + (e & 1);
-          x[e] = t < now.len ? sc[e >> 1][r * 2 + (e & 1)] * p.qscale : -INFINITY;
+          const int32_t t = (e >> 1) * 8 + 2 * tq + (e & 1);
+          x[e] = t < left ? sc[e >> 1][r * 2 + (e & 1)] * p.qscale : -INFINITY;
         }
         float bm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
         bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
         const float m_new = fmaxf(m_run[r], bm);
-        const float corr = exp2_approx(m_run[r] - m_new);
-        m_run[r] = m_new;
+        if (__any_sync(0xffffffffu, m_new != m_run[r])) {
+          const float corr = exp2_approx(m_run[r] - m_new);
+          m_run[r] = m_new;
+          l_run[r] *= corr;
+#pragma unroll
+          for (int j = 0; j < NDT; ++j) {
+            o[j][r * 2] *= corr;
+            o[j][r * 2 + 1] *= corr;
+          }
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e] - m_new);
-        l_run[r] = l_run[r] * corr + (x[0] + x[1]) + (x[2] + x[3]);
-#pragma unroll
-        for (int j = 0; j < NDT; ++j) {
-          o[j][r * 2] *= corr;
-          o[j][r * 2 + 1] *= corr;
-        }
+        l_run[r] += (x[0] + x[1]) + (x[2] + x[3]);
         pa[r] = float2_to_pair<T>(x[0], x[1]);
         pa[2 + r] = float2_to_pair<T>(x[2], x[3]);
       }
@@ -424,7 +461,7 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
       // Four chains a dot product keep its rounding error (which the exponential
       // turns into a relative one) at that of 8- or 16-term sums.
       const int tok = lane & 15, half = lane >> 4;
-      const bool live = t0 + tok < now.len;
+      const bool live = tok < left;
       float4 kf[CHUNKS / 2];
 #pragma unroll
       for (int c = 0; c < CHUNKS / 2; ++c)
@@ -447,16 +484,19 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
         float bm = live ? x * p.qscale : -FLT_MAX;
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, w));
-        const float m_new = fmaxf(m_run[r], bm);
-        const float corr = exp2f(m_run[r] - m_new);
-        m_run[r] = m_new;
-        s[r] = live ? exp2f(fmaf(x, p.qscale, -m_new)) : 0.f;
-        l_run[r] = l_run[r] * corr + (half == 0 ? s[r] : 0.f);  // one of the two copies counts
+        const float m_new = fmaxf(m_run[r], bm);  // the same in every lane
+        if (m_new != m_run[r]) {
+          const float corr = exp2f(m_run[r] - m_new);
+          m_run[r] = m_new;
+          l_run[r] *= corr;
 #pragma unroll
-        for (int e = 0; e < E; ++e) accf[r][e] *= corr;
+          for (int e = 0; e < E; ++e) accf[r][e] *= corr;
+        }
+        s[r] = live ? exp2f(fmaf(x, p.qscale, -m_new)) : 0.f;
+        l_run[r] += half == 0 ? s[r] : 0.f;  // one of the two copies counts
       }
 #pragma unroll 4
-      for (int t = 0; t < kWarpTokens; ++t) {
+      for (int t = 0; t < kTileTokens; ++t) {
         float vf[E];
         const uint32_t a = vb + swz<C::ROW_BYTES>(t, (lane * E) / 4) + ((lane * E) % 4) * 4;
         if constexpr (E == 4) {
@@ -479,157 +519,186 @@ __global__ void __launch_bounds__(kPagedThreads, 2)
     if (++stage == C::STAGES) stage = 0;
 
     // ---- the item, or this share's part of it, ends here
-    if (now.tile + 1 == now.tiles || u + 1 == ntiles) {
-      const int64_t item = static_cast<int64_t>(now.b) * p.hkv + now.head;
-      // Tiles of the item before this share, and whether it goes on after it.
-      const int64_t seg_tiles = min(static_cast<int64_t>(now.tile) + 1, u + 1);
-      const bool starts = seg_tiles == now.tile + 1, ends = now.tile + 1 == now.tiles;
-      const int part = 2 * static_cast<int>(blockIdx.x) + (first_segment ? 0 : 1);
-      if (starts && threadIdx.x == 0) {
+    const bool ends = now.tile + 1 == now.tiles;
+    if (ends || now.u + 1 == u1) {
+      const bool starts = now.u - now.tile >= u0;  // the share has the item's first tile
+      const bool whole = starts && ends;
+      const int part = 2 * me + (first_segment ? 0 : 1);
+      if (starts && lane == 0) {
+        const int64_t item = static_cast<int64_t>(now.b) * p.hkv + now.head;
         p.joins[item * 2] = ends ? -1 : part;
         p.joins[item * 2 + 1] =
-            static_cast<int32_t>((u0 + u - now.tile + now.tiles - 1) / share);
+            static_cast<int32_t>((now.u - now.tile + now.tiles - 1) / share);
       }
+      T* op = static_cast<T*>(p.out) + now.b * p.out_batch +
+              static_cast<int64_t>(now.head) * G * p.out_head;
+      float* wp = p.ws + static_cast<int64_t>(part) * G * D;
+      float* ml = p.ws + static_cast<int64_t>(2 * p.warps) * G * D + static_cast<int64_t>(part) * G * 2;
+      if constexpr (MMA) {
 #pragma unroll
-      for (int h8 = 0; h8 < (GMAX + 7) / 8; ++h8) {  // 8 heads at a time
-        const int heads = min(8, G - h8 * 8);
-        if (heads <= 0) break;
-        __syncthreads();  // the join buffers are free
-        if constexpr (MMA) {
-          float l = l_run[h8];
+        for (int r = 0; r < NR; ++r) {
+          float l = l_run[r];
           l += __shfl_xor_sync(0xffffffffu, l, 1);
           l += __shfl_xor_sync(0xffffffffu, l, 2);
-          if (g < heads) {
+          const int row = g + r * 8;
+          if (row >= G) continue;
+          if (whole) {
+            const float inv = 1.f / l;
 #pragma unroll
             for (int j = 0; j < NDT; ++j)
-              *reinterpret_cast<float2*>(sm_acc + (warp * 8 + g) * D + j * 8 + 2 * tq) =
-                  make_float2(o[j][h8 * 2], o[j][h8 * 2 + 1]);
-            if (tq == 0) {
-              sm_m[warp * 8 + g] = m_run[h8];
-              sm_l[warp * 8 + g] = l;
-            }
-          }
-        } else {
+              *reinterpret_cast<uint32_t*>(op + row * p.out_head + j * 8 + 2 * tq) =
+                  float2_to_pair<T>(o[j][r * 2] * inv, o[j][r * 2 + 1] * inv);
+          } else {
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const int row = h8 * 8 + r;
-            if (r >= heads) continue;
-            float l = l_run[row];
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) sm_acc[(warp * 8 + r) * D + lane * E + e] = accf[row][e];
-            if (lane == 0) {
-              sm_m[warp * 8 + r] = m_run[row];
-              sm_l[warp * 8 + r] = l;
-            }
+            for (int j = 0; j < NDT; ++j)
+              *reinterpret_cast<float2*>(wp + row * D + j * 8 + 2 * tq) =
+                  make_float2(o[j][r * 2], o[j][r * 2 + 1]);
+            if (tq == 0) *reinterpret_cast<float2*>(ml + row * 2) = make_float2(m_run[r], l);
           }
         }
-        __syncthreads();
-        for (int i = static_cast<int>(threadIdx.x); i < heads * D; i += kPagedThreads) {
-          const int r = i / D, d = i % D, row = h8 * 8 + r;
-          float mx = -FLT_MAX;
+      } else {
 #pragma unroll
-          for (int w = 0; w < kPagedWarps; ++w) mx = fmaxf(mx, sm_m[w * 8 + r]);
-          float num = 0.f, den = 0.f;
+        for (int r = 0; r < GMAX; ++r) {
+          if (r >= G) continue;
+          float l = l_run[r];
 #pragma unroll
-          for (int w = 0; w < kPagedWarps; ++w) {
-            const float f = exp2f(sm_m[w * 8 + r] - mx);
-            num = fmaf(sm_acc[(w * 8 + r) * D + d], f, num);
-            den = fmaf(sm_l[w * 8 + r], f, den);
-          }
-          if (starts && ends) {
-            T* op = static_cast<T*>(p.out) + now.b * p.out_batch +
-                    (static_cast<int64_t>(now.head) * G + row) * p.out_head;
-            op[d] = from_float<T>(num / den);
-          } else {
-            p.ws[(static_cast<int64_t>(part) * G + row) * D + d] = num;
-            if (d == 0) {
-              float* ml = p.ws + static_cast<int64_t>(2 * p.ctas) * G * D +
-                          (static_cast<int64_t>(part) * G + row) * 2;
-              ml[0] = mx;
-              ml[1] = den;
-            }
-          }
+          for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (whole)
+              op[r * p.out_head + lane * E + e] = from_float<T>(accf[r][e] / l);
+            else
+              wp[r * D + lane * E + e] = accf[r][e];
+          if (!whole && lane == 0) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(m_run[r], l);
         }
       }
       fresh = true;
       first_segment = false;
     }
-    if (u + 1 < ntiles) advance(p, now);
+    advance(p, now);
   }
 }
 
 // Joins the parts of every item that was cut, in share order, and writes the
-// zeros of empty sequences.  One CTA per (KV head, sequence), a thread per
-// (head, dim).
-template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedDecodeParams p, int D) {
+// zeros of empty sequences.  One CTA per (query head, sequence): a warp takes
+// every fourth part, a lane D / 32 dims; the loads of the parts do not depend on
+// one another, and the warps meet in shared memory.
+template <typename T, int D>
+__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDecodeParams p) {
+  constexpr int E = D / 32;
+  __shared__ float sm_acc[kPagedWarps][D];
+  __shared__ float2 sm_ml[kPagedWarps];
   griddep_launch_dependents();
   griddep_wait();
-  const int head = blockIdx.x, b = blockIdx.y;
-  const int64_t item = static_cast<int64_t>(b) * p.hkv + head;
-  T* op = static_cast<T*>(p.out) + b * p.out_batch + static_cast<int64_t>(head) * p.group * p.out_head;
-  if (p.seq_lens[b] <= 0) {
-    for (int i = static_cast<int>(threadIdx.x); i < p.group * D; i += blockDim.x)
-      op[(i / D) * p.out_head + i % D] = from_float<T>(0.f);
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int G = p.group, head = h / G, row = h - head * G;
+  T* op = static_cast<T*>(p.out) + b * p.out_batch + h * p.out_head;
+  const int2 join =
+      *reinterpret_cast<const int2*>(p.joins + (static_cast<int64_t>(b) * p.hkv + head) * 2);
+  if (p.seq_lens[b] <= 0 || p.kv.max_pages == 0) {
+    for (int d = static_cast<int>(threadIdx.x); d < D; d += kPagedThreads)
+      op[d] = from_float<T>(0.f);
     return;
   }
-  const int first = p.joins[item * 2];
-  if (first < 0) return;
-  const int last = p.joins[item * 2 + 1];  // CTA of the last part; its slot is the CTA's first
-  const int c0 = first / 2, n = last - c0 + 1;
-  const float* ml = p.ws + static_cast<int64_t>(2 * p.ctas) * p.group * D;
-  for (int i = static_cast<int>(threadIdx.x); i < p.group * D; i += blockDim.x) {
-    const int row = i / D, d = i % D;
-    float mx = -FLT_MAX;
-    for (int s = 0; s < n; ++s) {
-      const int64_t part = s == 0 ? first : 2 * (c0 + s);
-      mx = fmaxf(mx, ml[(part * p.group + row) * 2]);
+  if (join.x < 0) return;
+  // Parts: the first, then the first slots of the warps up to the last.
+  const int w0 = join.x / 2, n = join.y - w0 + 1;
+  const float* mls = p.ws + static_cast<int64_t>(2 * p.warps) * G * D;
+  float acc[E], mx = -FLT_MAX, den = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  constexpr int U = 4;
+  for (int s0 = warp; s0 < n; s0 += U * kPagedWarps) {
+    float2 ml[U];
+    float x[U][E];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int s = s0 + i * kPagedWarps;
+      ml[i] = make_float2(-FLT_MAX, 0.f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[i][e] = 0.f;
+      if (s < n) {
+        const int64_t at = static_cast<int64_t>(s == 0 ? join.x : 2 * (w0 + s)) * G + row;
+        ml[i] = *reinterpret_cast<const float2*>(mls + at * 2);
+        if constexpr (E == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p.ws + at * D + lane * 4);
+          x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(p.ws + at * D + lane * 2);
+          x[i][0] = v.x; x[i][1] = v.y;
+        }
+      }
     }
-    float num = 0.f, den = 0.f;
-    for (int s = 0; s < n; ++s) {
-      const int64_t part = s == 0 ? first : 2 * (c0 + s);
-      const float f = exp2f(ml[(part * p.group + row) * 2] - mx);
-      num = fmaf(p.ws[(part * p.group + row) * D + d], f, num);
-      den = fmaf(ml[(part * p.group + row) * 2 + 1], f, den);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float m_new = fmaxf(mx, ml[i].x), c = exp2f(mx - m_new), f = exp2f(ml[i].x - m_new);
+      mx = m_new;
+      den = fmaf(ml[i].y, f, den * c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(x[i][e], f, acc[e] * c);
     }
-    op[row * p.out_head + d] = from_float<T>(num / den);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sm_acc[warp][lane * E + e] = acc[e];
+  if (lane == 0) sm_ml[warp] = make_float2(mx, den);
+  __syncthreads();
+  for (int d = static_cast<int>(threadIdx.x); d < D; d += kPagedThreads) {
+    float m = -FLT_MAX;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) m = fmaxf(m, sm_ml[w].x);
+    float num = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) {
+      const float f = exp2f(sm_ml[w].x - m);
+      num = fmaf(sm_acc[w][d], f, num);
+      sum = fmaf(sm_ml[w].y, f, sum);
+    }
+    op[d] = from_float<T>(num / sum);
   }
 }
 
 // ------------------------------------------------------------------ host side
 
-// Every CTA resident (PagedCfg::CTAS_PER_SM of them on an SM), and no more of
-// them than there can be tiles.
+// The least share.  16-bit: a part costs about what reading two tiles does.  fp32:
+// the scores take longer than the part.
+static int paged_least(int dtype) { return dtype == FRN_DTYPE_F32 ? 1 : 4; }
+
+// Every CTA resident, and no more warps than there can be shares.
 static int paged_ctas(int dtype, int64_t batch, int64_t hkv, int64_t d, int64_t capacity, int sms) {
-  const int64_t resident = (dtype == FRN_DTYPE_F32 && d == 128 ? 1 : 2) * static_cast<int64_t>(sms);
-  const int64_t most = batch * hkv * ((capacity + kTileTokens - 1) / kTileTokens);
+  const int64_t resident =
+      static_cast<int64_t>(paged_ctas_per_sm(dtype == FRN_DTYPE_F32, static_cast<int>(d))) * sms;
+  const int64_t tiles = batch * hkv * ((capacity + kTileTokens - 1) / kTileTokens);
+  // A share has at least one item or `least` tiles of one.
+  const int64_t least = paged_least(dtype);
+  const int64_t shares = batch * hkv * ((tiles / (batch * hkv) + least - 1) / least);
+  const int64_t most = (shares + kPagedWarps - 1) / kPagedWarps;
   return static_cast<int>(most < resident ? (most > 0 ? most : 1) : resident);
 }
 
 size_t paged_decode_workspace(int dtype, int64_t batch, int64_t hq, int64_t hkv, int64_t d,
                               int64_t capacity, int sms) {
-  const int64_t c = paged_ctas(dtype, batch, hkv, d, capacity, sms);
-  const int64_t floats = 2 * c * (hq / hkv) * (d + 2);
+  const int64_t warps = kPagedWarps * static_cast<int64_t>(paged_ctas(dtype, batch, hkv, d, capacity, sms));
+  const int64_t floats = 2 * warps * (hq / hkv) * (d + 2);
   return static_cast<size_t>((floats + 2 * batch * hkv) * 4);
 }
 
 template <typename T, int D, int GMAX>
 static int launch_paged(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaStream_t stream) {
   using C = PagedCfg<T, D, GMAX>;
-  auto kern = paged_decode_kernel<T, D, GMAX>;
+  const bool uni = g.kv.page_size % kTileTokens == 0;
+  auto kern = uni ? paged_decode_kernel<T, D, GMAX, true> : paged_decode_kernel<T, D, GMAX, false>;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return set_cuda_error("cudaGetDevice");
-  static bool ready[kMaxDevices] = {};
-  if (dev >= kMaxDevices || !ready[dev]) {
+  static bool ready[2][kMaxDevices] = {};
+  if (dev >= kMaxDevices || !ready[uni][dev]) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
     if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(paged decode)", e);
-    if (dev < kMaxDevices) ready[dev] = true;
+    if (dev < kMaxDevices) ready[uni][dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.warps / kPagedWarps));
   cfg.blockDim = dim3(kPagedThreads);
   cfg.dynamicSmemBytes = C::SMEM_BYTES;
   cfg.stream = stream;
@@ -640,10 +709,9 @@ static int launch_paged(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaS
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return set_cuda_error("launch paged_decode", e);
-  cfg.gridDim = dim3(static_cast<unsigned>(g.kv.num_kv_heads), static_cast<unsigned>(g.batch));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<unsigned>(g.num_q_heads), static_cast<unsigned>(g.batch));
   cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, p, D);
+  e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, p);
   if (e != cudaSuccess) return set_cuda_error("launch paged_join", e);
   return 0;
 }
@@ -673,11 +741,12 @@ int run_paged_decode(const PagedDecodeProblem& g, cudaStream_t stream) {
   p.batch = static_cast<int32_t>(g.batch);
   p.hkv = static_cast<int32_t>(g.kv.num_kv_heads);
   p.group = static_cast<int32_t>(g.num_q_heads / g.kv.num_kv_heads);
-  p.ctas = paged_ctas(g.dtype, g.batch, g.kv.num_kv_heads, g.kv.head_dim,
-                      g.kv.max_pages * g.kv.page_size, sm_count(dev));
+  p.least = paged_least(g.dtype);
+  p.warps = kPagedWarps * paged_ctas(g.dtype, g.batch, g.kv.num_kv_heads, g.kv.head_dim,
+                                     g.kv.max_pages * g.kv.page_size, sm_count(dev));
   p.ws = static_cast<float*>(g.workspace);
   p.joins = reinterpret_cast<int32_t*>(
-      p.ws + static_cast<int64_t>(2 * p.ctas) * p.group * (g.kv.head_dim + 2));
+      p.ws + static_cast<int64_t>(2 * p.warps) * p.group * (g.kv.head_dim + 2));
   p.qscale = g.scale * 1.4426950408889634f;  // log2(e): the softmax runs in base 2
   switch (g.dtype) {
     case FRN_DTYPE_BF16: return launch_paged_d<__nv_bfloat16>(g, p, stream);
