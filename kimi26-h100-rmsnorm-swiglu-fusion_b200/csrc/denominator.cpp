@@ -328,6 +328,7 @@ void kv_pages_copy(const std::vector<at::Tensor>& pools, const std::vector<int64
   const at::Tensor& first = pools[0];
   TORCH_CHECK(first.dim() >= 2, name, ": a pool must be [num_pages, ...]");
   std::vector<void*> ptrs;
+  ptrs.reserve(pools.size());
   for (const at::Tensor& p : pools) {
     TORCH_CHECK(p.is_cuda(), "All tensors must be on CUDA");
     TORCH_CHECK(p.sizes() == first.sizes() && p.strides() == first.strides() &&
@@ -335,9 +336,12 @@ void kv_pages_copy(const std::vector<at::Tensor>& pools, const std::vector<int64
                 name, ": pools must share shape, strides, element size and device");
     ptrs.push_back(p.data_ptr());
   }
-  TORCH_CHECK(first.size(0) == 0 || first.select(0, 0).is_non_overlapping_and_dense(), name,
-              ": a page must be one dense block");
+  TORCH_CHECK(first.is_contiguous() || first.size(0) == 0 ||
+                  first.select(0, 0).is_non_overlapping_and_dense(),
+              name, ": a page must be one dense block");
   std::vector<int32_t> from, to;
+  from.reserve(src.size());
+  to.reserve(src.size());
   for (size_t i = 0; i < src.size(); ++i) {
     TORCH_CHECK(src[i] >= 0 && src[i] < first.size(0) && dst[i] >= 0 && dst[i] < first.size(0),
                 name, ": copy ", i, ": page ", src[i], " -> ", dst[i], " outside the ",

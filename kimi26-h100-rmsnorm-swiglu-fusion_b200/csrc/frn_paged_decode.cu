@@ -31,7 +31,9 @@
 // Arithmetic.  bf16 / fp16: the query heads of a group are the rows of 16x8x16
 // MMAs (S = Q K^T, O += P V; up to 16 heads), online softmax in base 2 on the
 // fragments, statistics and accumulators in fp32; P is rounded to the input
-// type for the second product, its row sums are not.  fp32: CUDA cores, one
+// type for the second product, its row sums are not (a second product with what
+// the rounding leaves would take the error from 1.4 times the output's own
+// rounding to that, and costs 2 to 4% of the time).  fp32: CUDA cores, one
 // token a lane for the scores, head dims across lanes for the output.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -60,7 +62,9 @@ struct PagedDecodeParams {
   const int32_t* seq_lens;
   float* ws;       // [2 * warps][G][D] accumulators, then [2 * warps][G][2] (max, sum)
   int32_t* joins;  // [batch * Hkv][2] first part (-1: nothing to join), last warp
-  int32_t batch, hkv, group, warps, least;
+  int32_t batch, hkv, group, warps;
+  int32_t least, least_share;  // tiles that an item counts as, and that a share has, at least
+  int32_t join_rows;  // query heads of a CTA of the join: 1 or 4
   float qscale;    // scale * log2(e): the softmax runs in base 2
 };
 
@@ -89,6 +93,17 @@ __device__ __forceinline__ void cp_async_commit() {
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Two fp32 multiply-adds an instruction.
+__device__ __forceinline__ float2 fma_f32x2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -244,7 +259,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
   // ---- the warps' shares of the tiles, and where they start
   int64_t before, own;
   const int64_t total = scan_tiles(p, sm_warp, &before, &own);
-  const int64_t share = max((total + p.warps - 1) / p.warps, static_cast<int64_t>(p.least));
+  const int64_t share = max((total + p.warps - 1) / p.warps, static_cast<int64_t>(p.least_share));
   const int me = static_cast<int>(blockIdx.x) * kPagedWarps + warp;  // this warp's number
   if (own > 0) {
     // The shares of this CTA that start within this thread's run of sequences.
@@ -466,20 +481,21 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
 #pragma unroll
       for (int c = 0; c < CHUNKS / 2; ++c)
         kf[c] = ld_shared_v4f(kb + swz<C::ROW_BYTES>(tok, half * (CHUNKS / 2) + c));
+      __syncwarp();  // K is read: its place takes the probabilities, [token][head]
       float s[GMAX];
 #pragma unroll
       for (int r = 0; r < GMAX; ++r) {
+        s[r] = 0.f;
         if (r >= G) continue;
         const float4* qf = reinterpret_cast<const float4*>(sm_q + r * D) + half * (CHUNKS / 2);
-        float4 d = make_float4(0.f, 0.f, 0.f, 0.f);
+        float2 d0 = make_float2(0.f, 0.f), d1 = d0;
 #pragma unroll
         for (int c = 0; c < CHUNKS / 2; ++c) {
-          d.x = fmaf(qf[c].x, kf[c].x, d.x);
-          d.y = fmaf(qf[c].y, kf[c].y, d.y);
-          d.z = fmaf(qf[c].z, kf[c].z, d.z);
-          d.w = fmaf(qf[c].w, kf[c].w, d.w);
+          const float4 q4 = qf[c];
+          d0 = fma_f32x2(make_float2(q4.x, q4.y), make_float2(kf[c].x, kf[c].y), d0);
+          d1 = fma_f32x2(make_float2(q4.z, q4.w), make_float2(kf[c].z, kf[c].w), d1);
         }
-        float x = (d.x + d.y) + (d.z + d.w);
+        float x = (d0.x + d0.y) + (d1.x + d1.y);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         float bm = live ? x * p.qscale : -FLT_MAX;
 #pragma unroll
@@ -495,23 +511,38 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
         s[r] = live ? exp2f(fmaf(x, p.qscale, -m_new)) : 0.f;
         l_run[r] += half == 0 ? s[r] : 0.f;  // one of the two copies counts
       }
+      if (half == 0) {
+#pragma unroll
+        for (int r = 0; r < GMAX; r += 4)
+          st_shared_v4(kb + (tok * GMAX + r) * 4, __float_as_uint(s[r]), __float_as_uint(s[r + 1]),
+                       __float_as_uint(s[r + 2]), __float_as_uint(s[r + 3]));
+      }
+      __syncwarp();
 #pragma unroll 4
       for (int t = 0; t < kTileTokens; ++t) {
-        float vf[E];
+        float2 vf[E / 2];
         const uint32_t a = vb + swz<C::ROW_BYTES>(t, (lane * E) / 4) + ((lane * E) % 4) * 4;
         if constexpr (E == 4) {
           const float4 v4 = ld_shared_v4f(a);
-          vf[0] = v4.x; vf[1] = v4.y; vf[2] = v4.z; vf[3] = v4.w;
+          vf[0] = make_float2(v4.x, v4.y);
+          vf[1] = make_float2(v4.z, v4.w);
         } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) vf[e] = ld_shared_f32(a + e * 4);
+          vf[0] = make_float2(ld_shared_f32(a), ld_shared_f32(a + 4));
         }
 #pragma unroll
-        for (int r = 0; r < GMAX; ++r) {
-          if (r >= G) continue;
-          const float pt = __shfl_sync(0xffffffffu, s[r], t);
+        for (int r4 = 0; r4 < GMAX; r4 += 4) {
+          if (r4 >= G) continue;
+          const float4 p4 = ld_shared_v4f(kb + (t * GMAX + r4) * 4);
+          const float pt[4] = {p4.x, p4.y, p4.z, p4.w};
 #pragma unroll
-          for (int e = 0; e < E; ++e) accf[r][e] = fmaf(pt, vf[e], accf[r][e]);
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+              const float2 w = fma_f32x2(make_float2(pt[r], pt[r]), vf[e / 2],
+                                         make_float2(accf[r4 + r][e], accf[r4 + r][e + 1]));
+              accf[r4 + r][e] = w.x;
+              accf[r4 + r][e + 1] = w.y;
+            }
         }
       }
     }
@@ -579,53 +610,36 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
   }
 }
 
-// Joins the parts of every item that was cut, in share order, and writes the
-// zeros of empty sequences.  One CTA per (query head, sequence): a warp takes
-// every fourth part, a lane D / 32 dims; the loads of the parts do not depend on
-// one another, and the warps meet in shared memory.
-template <typename T, int D>
-__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDecodeParams p) {
-  constexpr int E = D / 32;
-  __shared__ float sm_acc[kPagedWarps][D];
-  __shared__ float2 sm_ml[kPagedWarps];
-  griddep_launch_dependents();
-  griddep_wait();
-  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int G = p.group, head = h / G, row = h - head * G;
-  T* op = static_cast<T*>(p.out) + b * p.out_batch + h * p.out_head;
-  const int2 join =
-      *reinterpret_cast<const int2*>(p.joins + (static_cast<int64_t>(b) * p.hkv + head) * 2);
-  if (p.seq_lens[b] <= 0 || p.kv.max_pages == 0) {
-    for (int d = static_cast<int>(threadIdx.x); d < D; d += kPagedThreads)
-      op[d] = from_float<T>(0.f);
-    return;
-  }
-  if (join.x < 0) return;
-  // Parts: the first, then the first slots of the warps up to the last.
-  const int w0 = join.x / 2, n = join.y - w0 + 1;
-  const float* mls = p.ws + static_cast<int64_t>(2 * p.warps) * G * D;
-  float acc[E], mx = -FLT_MAX, den = 0.f;
+// Sum of the parts s0, s0 + step, ... of one row, brought to their largest
+// maximum; a lane holds D / 32 dims.  The loads of the parts do not depend on one
+// another.
+template <int E>
+__device__ __forceinline__ void join_parts(const PagedDecodeParams& p, const float* mls, int first,
+                                           int w0, int n, int s0, int step, int row, int lane,
+                                           float (&acc)[E], float& mx, float& den) {
+  constexpr int U = 4;
+  mx = -FLT_MAX;
+  den = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  constexpr int U = 4;
-  for (int s0 = warp; s0 < n; s0 += U * kPagedWarps) {
+  for (; s0 < n; s0 += U * step) {
     float2 ml[U];
     float x[U][E];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int s = s0 + i * kPagedWarps;
+      const int s = s0 + i * step;
       ml[i] = make_float2(-FLT_MAX, 0.f);
 #pragma unroll
       for (int e = 0; e < E; ++e) x[i][e] = 0.f;
       if (s < n) {
-        const int64_t at = static_cast<int64_t>(s == 0 ? join.x : 2 * (w0 + s)) * G + row;
+        // The first part, then the first slots of the warps up to the last.
+        const int64_t at = static_cast<int64_t>(s == 0 ? first : 2 * (w0 + s)) * p.group + row;
         ml[i] = *reinterpret_cast<const float2*>(mls + at * 2);
         if constexpr (E == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p.ws + at * D + lane * 4);
+          const float4 v = *reinterpret_cast<const float4*>(p.ws + at * (E * 32) + lane * 4);
           x[i][0] = v.x; x[i][1] = v.y; x[i][2] = v.z; x[i][3] = v.w;
         } else {
-          const float2 v = *reinterpret_cast<const float2*>(p.ws + at * D + lane * 2);
+          const float2 v = *reinterpret_cast<const float2*>(p.ws + at * (E * 32) + lane * 2);
           x[i][0] = v.x; x[i][1] = v.y;
         }
       }
@@ -639,38 +653,85 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDe
       for (int e = 0; e < E; ++e) acc[e] = fmaf(x[i][e], f, acc[e] * c);
     }
   }
+}
+
+// Joins the parts of every item that was cut, in share order, and writes the
+// zeros of empty sequences.  A CTA has join_rows query heads of one KV head:
+// four where there are many rows (and so few parts of each), a warp each; one
+// where there are few.  An item of many parts is joined by the four warps
+// together, row by row.
+template <typename T, int D>
+__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDecodeParams p) {
+  constexpr int E = D / 32;
+  __shared__ float sm_acc[kPagedWarps][D];
+  __shared__ float2 sm_ml[kPagedWarps];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  const int G = p.group, per_head = (G + p.join_rows - 1) / p.join_rows;
+  const int head = blockIdx.x / per_head, b = blockIdx.y;
+  const int row0 = (blockIdx.x - head * per_head) * p.join_rows;
+  const int rows = min(p.join_rows, G - row0);
+  T* op = static_cast<T*>(p.out) + b * p.out_batch +
+          (static_cast<int64_t>(head) * G + row0) * p.out_head;
+  const int2 join =
+      *reinterpret_cast<const int2*>(p.joins + (static_cast<int64_t>(b) * p.hkv + head) * 2);
+  if (p.seq_lens[b] <= 0 || p.kv.max_pages == 0) {
+    for (int i = static_cast<int>(threadIdx.x); i < rows * D; i += kPagedThreads)
+      op[(i / D) * p.out_head + i % D] = from_float<T>(0.f);
+    return;
+  }
+  if (join.x < 0) return;
+  const int w0 = join.x / 2, n = join.y - w0 + 1;
+  const float* mls = p.ws + static_cast<int64_t>(2 * p.warps) * G * D;
+  float acc[E], mx, den;
+  if (rows > 1 && n <= 16) {
+    if (warp < rows) {
+      join_parts<E>(p, mls, join.x, w0, n, 0, 1, row0 + warp, lane, acc, mx, den);
 #pragma unroll
-  for (int e = 0; e < E; ++e) sm_acc[warp][lane * E + e] = acc[e];
-  if (lane == 0) sm_ml[warp] = make_float2(mx, den);
-  __syncthreads();
-  for (int d = static_cast<int>(threadIdx.x); d < D; d += kPagedThreads) {
-    float m = -FLT_MAX;
-#pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) m = fmaxf(m, sm_ml[w].x);
-    float num = 0.f, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) {
-      const float f = exp2f(sm_ml[w].x - m);
-      num = fmaf(sm_acc[w][d], f, num);
-      sum = fmaf(sm_ml[w].y, f, sum);
+      for (int e = 0; e < E; ++e)
+        op[warp * p.out_head + lane * E + e] = from_float<T>(acc[e] / den);
     }
-    op[d] = from_float<T>(num / sum);
+    return;
+  }
+  for (int r = 0; r < rows; ++r) {
+    join_parts<E>(p, mls, join.x, w0, n, warp, kPagedWarps, row0 + r, lane, acc, mx, den);
+    if (r > 0) __syncthreads();  // the last row's meeting is over
+#pragma unroll
+    for (int e = 0; e < E; ++e) sm_acc[warp][lane * E + e] = acc[e];
+    if (lane == 0) sm_ml[warp] = make_float2(mx, den);
+    __syncthreads();
+    for (int d = static_cast<int>(threadIdx.x); d < D; d += kPagedThreads) {
+      float m = -FLT_MAX;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) m = fmaxf(m, sm_ml[w].x);
+      float num = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kPagedWarps; ++w) {
+        const float f = exp2f(sm_ml[w].x - m);
+        num = fmaf(sm_acc[w][d], f, num);
+        sum = fmaf(sm_ml[w].y, f, sum);
+      }
+      op[r * p.out_head + d] = from_float<T>(num / sum);
+    }
   }
 }
 
 // ------------------------------------------------------------------ host side
 
-// The least share.  16-bit: a part costs about what reading two tiles does.  fp32:
-// the scores take longer than the part.
+// 16-bit: an item's queries and end cost about what four tiles do, a part what two
+// do (one sequence of 1000 tokens: 8.9 us with shares of two, 10.2 with four; 64
+// sequences of 1 to 8192: 48 us where an item counts as two at least, 45 with
+// four).  fp32: the scores of a tile take longer than either.
 static int paged_least(int dtype) { return dtype == FRN_DTYPE_F32 ? 1 : 4; }
+static int paged_least_share(int dtype) { return dtype == FRN_DTYPE_F32 ? 1 : 2; }
 
 // Every CTA resident, and no more warps than there can be shares.
 static int paged_ctas(int dtype, int64_t batch, int64_t hkv, int64_t d, int64_t capacity, int sms) {
   const int64_t resident =
       static_cast<int64_t>(paged_ctas_per_sm(dtype == FRN_DTYPE_F32, static_cast<int>(d))) * sms;
   const int64_t tiles = batch * hkv * ((capacity + kTileTokens - 1) / kTileTokens);
-  // A share has at least one item or `least` tiles of one.
-  const int64_t least = paged_least(dtype);
+  const int64_t least = paged_least_share(dtype);
   const int64_t shares = batch * hkv * ((tiles / (batch * hkv) + least - 1) / least);
   const int64_t most = (shares + kPagedWarps - 1) / kPagedWarps;
   return static_cast<int>(most < resident ? (most > 0 ? most : 1) : resident);
@@ -709,7 +770,9 @@ static int launch_paged(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaS
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess) return set_cuda_error("launch paged_decode", e);
-  cfg.gridDim = dim3(static_cast<unsigned>(g.num_q_heads), static_cast<unsigned>(g.batch));
+  cfg.gridDim = dim3(
+      static_cast<unsigned>(p.hkv * ((p.group + p.join_rows - 1) / p.join_rows)),
+      static_cast<unsigned>(g.batch));
   cfg.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, p);
   if (e != cudaSuccess) return set_cuda_error("launch paged_join", e);
@@ -741,7 +804,9 @@ int run_paged_decode(const PagedDecodeProblem& g, cudaStream_t stream) {
   p.batch = static_cast<int32_t>(g.batch);
   p.hkv = static_cast<int32_t>(g.kv.num_kv_heads);
   p.group = static_cast<int32_t>(g.num_q_heads / g.kv.num_kv_heads);
+  p.join_rows = g.batch * g.num_q_heads > 32 * sm_count(dev) ? 4 : 1;
   p.least = paged_least(g.dtype);
+  p.least_share = paged_least_share(g.dtype);
   p.warps = kPagedWarps * paged_ctas(g.dtype, g.batch, g.kv.num_kv_heads, g.kv.head_dim,
                                      g.kv.max_pages * g.kv.page_size, sm_count(dev));
   p.ws = static_cast<float*>(g.workspace);

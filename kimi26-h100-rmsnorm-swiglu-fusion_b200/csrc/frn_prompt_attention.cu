@@ -311,8 +311,9 @@ struct ItemFinder {
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       if (more) look(p, b0 + static_cast<int>(threadIdx.x & 31));
       int32_t part = 0;
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) part += max(0, __shfl_sync(0xffffffffu, blocks, i) - level);
+#pragma unroll 4
+      for (int i = 0; i < min(32, p.batch - b0); ++i)
+        part += max(0, __shfl_sync(0xffffffffu, blocks, i) - level);
       n += part;
     }
     return n;
