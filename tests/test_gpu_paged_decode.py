@@ -171,6 +171,7 @@ def test_streams_graphs_and_repeats():
 
 
 def test_python_surface():
+    from src.gqa_attention_forward import GQAPagedDecodeAttention
     from src.load_gqa_attention import gqa_attention_cuda as ops
 
     lens = [70, 0, 33]
@@ -180,6 +181,9 @@ def test_python_surface():
     ld = torch.tensor(lens, dtype=torch.int32, device=DEV)
     ref, spread = orc.paged_decode(q, k, v, table, torch.tensor(lens), 0.1)
     orc.assert_close(ops.gqa_paged_decode(qd, kd, vd, td, ld, 0.1), ref, spread)
+    module = GQAPagedDecodeAttention(8, 2, 128, scale=0.1)
+    orc.assert_close(module(qd, kd, vd, td, ld), ref, spread)
+    orc.assert_close(module(qd.flatten(1), kd, vd, td, ld), ref, spread)
     assert ops.gqa_paged_decode(qd[:0], kd, vd, td[:0], ld[:0], 0.1).shape == (0, 8, 128)
     for args, match in [((qd.half(), kd, vd, td, ld), "dtype"),
                         ((qd[:, :7], kd, vd, td, ld), "multiple of num_kv_heads"),

@@ -220,6 +220,7 @@ def test_streams_graphs_and_repeats():
 
 
 def test_python_surface():
+    from src.gqa_attention_forward import GQAPromptAttention
     from src.load_gqa_attention import gqa_attention_cuda as ops
 
     q, k, v, cu = make([60, 9], 4, 2, 128, 128, seed=1)
@@ -227,6 +228,9 @@ def test_python_surface():
     cud = torch.tensor(cu, dtype=torch.int32, device=DEV)
     qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
     orc.assert_close(ops.gqa_prompt_attention(qd, kd, vd, cud, 60, 0.1), ref, spread)
+    module = GQAPromptAttention(4, 2, 128, scale=0.1)
+    orc.assert_close(module(qd, kd, vd, cud, 60), ref, spread)
+    orc.assert_close(module(qd.flatten(1), kd.flatten(1), vd.flatten(1), cud, 60), ref, spread)
     # Layouts the kernel cannot read are copied first.
     odd = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (qd, kd, vd)]
     orc.assert_close(ops.gqa_prompt_attention(*odd, cud, 60, 0.1), ref, spread)
