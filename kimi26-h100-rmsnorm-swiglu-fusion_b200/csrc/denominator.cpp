@@ -9,6 +9,7 @@
 // fused_rmsnorm_swiglu (single-launch fused ops), the int8-weight path, and
 // device_error.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -277,13 +278,17 @@ at::Tensor gqa_paged_decode(const at::Tensor& q_in, const at::Tensor& k_pages,
   const int dt = dtype_code(q);
   const size_t need = frn_gqa_paged_decode_workspace_size(dt, q.size(0), q.size(1), c.num_kv_heads,
                                                           c.head_dim, c.page_size, c.max_pages);
-  const at::Tensor ws = at::empty({static_cast<int64_t>(need)}, q.options().dtype(at::kByte));
-  check_rc(frn_gqa_paged_decode_attention(dt, q.data_ptr(), stride_or(q, 0), stride_or(q, 1), &c,
-                                          seq_lens.data_ptr<int32_t>(), o.data_ptr(),
-                                          stride_or(o, 0), stride_or(o, 1), q.size(0), q.size(1),
-                                          static_cast<float>(scale), ws.data_ptr(), need,
-                                          stream_of(q)),
-           name);
+  // The workspace straight from torch's allocator: as a tensor it would take
+  // longer to make than the rest of the call.  Freed at once, it can only be
+  // given to later work of this stream.
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_of(q));
+  void* ws = c10::cuda::CUDACachingAllocator::raw_alloc_with_stream(need, stream);
+  const int rc = frn_gqa_paged_decode_attention(
+      dt, q.data_ptr(), stride_or(q, 0), stride_or(q, 1), &c, seq_lens.data_ptr<int32_t>(),
+      o.data_ptr(), stride_or(o, 0), stride_or(o, 1), q.size(0), q.size(1),
+      static_cast<float>(scale), ws, need, stream);
+  c10::cuda::CUDACachingAllocator::raw_delete(ws);
+  check_rc(rc, name);
   return o;
 }
 

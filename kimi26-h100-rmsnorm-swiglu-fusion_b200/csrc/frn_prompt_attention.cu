@@ -56,6 +56,7 @@ constexpr int kPromptThreads = 512;
 constexpr int kRows = 128;   // rows of a tile
 // Warps: 0-3 and 4-7 softmax of row tile 0 and 1, 8-11 output.
 constexpr int kOut = 8, kLoadQK = 12, kMma = 13, kLoadV = 15;
+constexpr int kAhead = 6;      // K/V tiles before its end that an item's successor is found
 constexpr int kItemSlots = 4;  // items that the scheduler is ahead
 constexpr float kLag = 8.f;  // log2 of the most that a probability may exceed 1
 
@@ -282,7 +283,7 @@ __device__ __forceinline__ void sequence_of(const PromptParams& p, int b, int32_
 struct ItemFinder {
   int32_t first, blocks, len;  // this lane's of the first 32 sequences
   int32_t below;               // the level is below this: it falls as the number grows
-  int64_t last;                // the last number looked for
+  int32_t last;                // the last number looked for
   bool more;                   // more than 32 sequences
 
   __device__ __forceinline__ void look(const PromptParams& p, int b) {
@@ -306,34 +307,32 @@ struct ItemFinder {
   }
 
   // F at this lane's level.
-  __device__ __forceinline__ int64_t count(const PromptParams& p, int32_t level) {
-    int64_t n = 0;
+  __device__ __forceinline__ int32_t count(const PromptParams& p, int32_t level) {
+    int32_t n = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       if (more) look(p, b0 + static_cast<int>(threadIdx.x & 31));
-      int32_t part = 0;
 #pragma unroll 4
       for (int i = 0; i < min(32, p.batch - b0); ++i)
-        part += max(0, __shfl_sync(0xffffffffu, blocks, i) - level);
-      n += part;
+        n += max(0, __shfl_sync(0xffffffffu, blocks, i) - level);
     }
     return n;
   }
 
-  __device__ __forceinline__ bool find(const PromptParams& p, int64_t index, PromptItem& item) {
+  __device__ __forceinline__ bool find(const PromptParams& p, int32_t index, PromptItem& item) {
     const int lane = static_cast<int>(threadIdx.x & 31);
     if (index < last) below = most(p);
     last = index;
     int32_t lo = 0, hi = below;  // F(lo) > index >= F(hi), if there is such an item
-    int64_t above = 0;           // F(hi)
+    int32_t above = 0;           // F(hi)
     bool first_round = true;
     while (hi - lo > 1 || first_round) {
       const int32_t step = (hi - lo + 31) / 32;
       const int32_t level = lo + lane * step;
-      const int64_t n = count(p, min(level, hi));
+      const int32_t n = count(p, min(level, hi));
       const uint32_t yes = __ballot_sync(0xffffffffu, level < hi && n > index);
       if (yes == 0) return false;
       const int top = 31 - __clz(yes);
-      const int64_t next = __shfl_sync(0xffffffffu, n, min(top + 1, 31));
+      const int32_t next = __shfl_sync(0xffffffffu, n, min(top + 1, 31));
       if (top < 31 && lo + (top + 1) * step < hi) {
         above = next;
         hi = lo + (top + 1) * step;
@@ -344,7 +343,7 @@ struct ItemFinder {
       first_round = false;
     }
     below = lo + 1;
-    int64_t k = index - above;
+    int32_t k = index - above;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       if (more) look(p, b0 + lane);
       uint32_t mask = __ballot_sync(0xffffffffu, blocks > lo);
@@ -550,15 +549,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
     } else if (warp == kLoadV) {
       // ---- items and loads of V.  The first item is the CTA's own number; then
-      // it takes those of CTAs that have not been launched yet, each when the
-      // loads of the one before are under way: earlier, and an item would wait
-      // here while another SM is idle.
+      // it takes those of CTAs that have not been launched yet, each a few tiles
+      // before the one before ends: earlier, and an item would wait here while
+      // another SM is idle; later, and this SM waits for its first tiles.
       bool ok = true, done = false;
       ItemFinder finder;
       finder.start(p);
-      const int64_t blocks = finder.count(p, 0);  // of all sequences, for one head
-      const int64_t per_group = blocks * p.heads_at_once;
-      int64_t last_group = -1;
+      // Blocks of all sequences, for one head.  Items are fewer than 2^31: their
+      // numbers are those of CTAs.
+      const int32_t blocks = finder.count(p, 0);
+      const int32_t per_group = max(1, blocks * p.heads_at_once);
+      int32_t last_group = -1;
       uint32_t answers = 0;
       auto ask = [&]() {
         fence_proxy_async_smem();  // the last answer has been read
@@ -568,31 +569,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           take_cta(answer, answer_full);
         }
       };
-      auto hear = [&](int64_t& index) {
+      auto hear = [&](int32_t& index) {
         ok = ok && mbar_wait(answer_full, answers++ & 1u, abort_flag, to);
         uint32_t cta = 0;
         const bool got = ok && taken_cta(answer, cta);
-        index = cta;
+        index = static_cast<int32_t>(cta);
         return got;
       };
       auto publish = [&](int32_t it) {
         if (done || !ok) return;
-        int64_t index = blockIdx.x;
+        int32_t index = static_cast<int32_t>(blockIdx.x);
         bool some = it == 0 || hear(index);
         if (!ok) return;
         const bool more = some;
         if (more) ask();
         PromptItem item;
         if (some) {
-          const int64_t group = blocks > 0 ? index / per_group : p.hkv;
-          const int32_t head0 = static_cast<int32_t>(min(group * p.heads_at_once,
-                                                         static_cast<int64_t>(p.hkv)));
+          const int32_t group = index / per_group;
+          const int32_t head0 = group * p.heads_at_once;
           const int32_t heads = min(p.heads_at_once, p.hkv - head0);
           if (group != last_group) finder.below = finder.most(p);
           last_group = group;
           index -= group * per_group;
-          some = heads > 0 && finder.find(p, index / heads, item);
-          item.kvh = head0 + (heads > 0 ? static_cast<int32_t>(index % heads) : 0);
+          const int32_t block = heads > 0 ? index / heads : 0;
+          some = heads > 0 && blocks > 0 && finder.find(p, block, item);
+          item.kvh = head0 + index - block * heads;
         }
         done = !some;
         if (done) item.len = 0;  // the end
@@ -621,8 +622,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
               tma_load_3d(smem + C::OFF_V + vs * C::V_BYTES + h * C::HALF, &tmap_v, &v_full[vs],
                           h * 64, item.kvh, item.first + j * kKeys);
           }
+          if (j == max(0, n - kAhead)) publish(it + 1);
         }
-        publish(it + 1);
       }
       if (*abort_flag) __nanosleep(20000);  // loads already issued may still be landing
     } else {
