@@ -10,8 +10,12 @@
 //          and the page lookup are dependent loads; one thread per token does
 //          them, not one per 16 bytes), then streams K and V in 16-byte
 //          pieces.
+//          21506 tokens (176 MB) take 30.6 us, 5.8 TB/s or 88% of a plain
+//          copy's rate; 64 tokens 1.9 us, a launch.
 // copy     the (src, dst) list and the pool pointers travel as kernel
 //          parameters: no upload and no workspace, so a fork is one launch.
+//          8 pages of 32 KB in 64 pools (34 MB) take 4.9 us, 1001 pages (4.2 GB)
+//          624 us, 6.7 TB/s.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -81,7 +85,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const AppendP
   __syncthreads();
   const int n = p.tokens_per_cta * p.row_vecs;
   // Pieces of K and V are loaded four at a time before any is stored: one at a
-  // time, 21506 tokens of 8 heads took 33 us instead of ...
+  // time, 21506 tokens of 8 heads of 128 took 32.8 us instead of 30.6.
   for (int i0 = static_cast<int>(threadIdx.x); i0 < n; i0 += kAppendThreads * kAppendVecs) {
     uint4 kv[kAppendVecs], vv[kAppendVecs];
     char* kd[kAppendVecs];

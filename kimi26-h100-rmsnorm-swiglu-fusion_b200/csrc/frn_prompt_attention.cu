@@ -18,7 +18,8 @@
 // keys and values would not fit L2 together come one group after the other.
 //
 // There is a CTA for each item; those that run take over the items of CTAs that
-// have not been launched, in that order.  Two row tiles an item take turns on the tensor core:
+// have not been launched, in that order.  Two row tiles an item take turns on the
+// tensor core:
 //   S_s = Q_s K_j^T   (128 rows x 128 keys, operands in shared memory)
 //   O_s += P_s V_j    (P_s from TMEM, where it overwrites S_s; V from shared
 //                      memory as it lies, keys being the slow dimension)
@@ -29,15 +30,28 @@
 // After a tile's last PV comes its first S of the next item, so that the loads
 // and first products of an item run under the end of the last.
 //
-// Roles: warps 0-3 and 4-7 the softmax and output of tile 0 and 1, warps 9 and
-// 10 their MMAs, warp 8 loads Q and K, warp 11 finds the items and loads V (whose
-// ring may be full while a K tile is needed).
+// Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, 8-11 the output of
+// both, 12 loads Q and K, 13 and 14 issue the MMAs of tile 0 and 1, 15 finds the
+// items and loads V (whose ring may be full while a K tile is needed).
 //
 // Softmax in base 2.  The maximum that scales the exponentials may lag the true
 // running maximum by up to 2^8 (kLag); O in TMEM is only rescaled, by the
 // warp whose rows need it, when the lag would grow beyond that.  The final
 // division makes the result independent of it.  P is rounded to the input type
 // for the second product; the row sums are of the unrounded values, in fp32.
+//
+// What bounds it.  Of a K/V tile and both row tiles the tensor core has 2048
+// clocks of work (D = 128), the special-function units 2048; a round takes 2840:
+// the way of one row tile from a finished S through its exponentials (1800), the
+// rest of PV and the next S (750) and two barriers (300).  One prompt of 8192
+// tokens, 32 / 8 heads of 128, bf16: 430 us (1270 TFLOP/s) in short runs at
+// 1.73 GHz, 490 to 510 us (1100 TFLOP/s) without pause, where the power limit
+// holds the clock at 1.49 GHz; MLA heads (192 / 128) 720 TFLOP/s, 24 packed
+// prompts of 16 to 1500 tokens 640 TFLOP/s (items of one to twelve tiles: the
+// first tile's maximum cannot be guessed, and both row tiles begin together).
+// Not adopted: a quarter or half of the exponentials by polynomial (no gain once
+// the registers sufficed, 2.5% at D = 64), two threads a row (the maximum has to
+// be agreed on: 611 us), spinning instead of suspended waits (3% slower).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -58,7 +72,8 @@ constexpr int kRows = 128;   // rows of a tile
 constexpr int kOut = 8, kLoadQK = 12, kMma = 13, kLoadV = 15;
 constexpr int kAhead = 6;      // K/V tiles before its end that an item's successor is found
 constexpr int kItemSlots = 4;  // items that the scheduler is ahead
-constexpr float kLag = 8.f;  // log2 of the most that a probability may exceed 1
+constexpr float kLag = 8.f;    // log2 of the most that a probability may exceed 1
+constexpr float kFloor = -1e30f;  // least first maximum: scores of -inf alone are not one
 
 // Two row tiles of one KV head: tokens from t0 on of the sequence in rows
 // [first, first + len).  len = 0: no more items.
@@ -71,8 +86,9 @@ struct PromptCfg {
   static constexpr int QH = DQK / 64, VH = DV / 64;  // 64-column halves (128-byte rows)
   // Keys of a K/V tile.  With 192 columns 96 of them, so that K and V tiles fit
   // twice beside the two Q tiles (with 128 a second V tile does not, and every
-  // tile waits for its V; with 64 a product of 64 x 16 keys takes 48 clocks of the
-  // tensor core where 32 would do, for its operands' shared-memory reads).
+  // tile waits for its V: 308 us for four sequences of 500 to 2048 tokens, 64
+  // heads, 289 with 96; with 64 a product takes 48 clocks of the tensor core where
+  // 32 would do, for its operands' shared-memory reads).
   static constexpr int KEYS = DQK == 192 ? 96 : 128;
   static constexpr int MOST = KEYS - 32;             // keys whose P is announced before the rest
   static constexpr int QHALF = kRows * 128;          // bytes of 128 rows x 64 columns
@@ -230,8 +246,8 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
 
 // True in one lane of a converged warp.  Unlike a test of the lane number this
 // tells the compiler that the branch is for a single thread, so that the MMA's
-// uniform operands need no loop over lanes (a PV of eight MMAs is issued in ...
-// cycles instead of 770).
+// uniform operands need no loop over lanes: the eight MMAs of a PV are issued in
+// 450 clocks instead of 770, the whole of 8192 tokens takes 586 us instead of 669.
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
   asm volatile(
@@ -1035,7 +1051,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             m_tile = fmaxf(m_tile, m2);
           }
           if (j == 0)
-            m_used = m_tile;
+            m_used = fmaxf(m_tile, kFloor);
           else if (__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag))
             move_max(m_tile);
 #pragma unroll
