@@ -1003,69 +1003,64 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             tmem_st_32x32b_x16(tm_o + b, o);
           }
         };
-        const int32_t least = t0 + warp_tok0 + 1 - j * kKeys;
-        if (j > 0 && least >= kKeys) {
-          // Every row sees the whole tile.  The first piece goes ahead with the
-          // maximum so far, while the tile's own is found; rarely, it has to be
-          // done again.
+        const int32_t least = t0 + warp_tok0 + 1 - j * kKeys;  // keys that every row sees
+        const int32_t most = t0 + warp_tok1 + 1 - j * kKeys;   // and that any row does
+        auto tile = [&](auto masked) {
+          constexpr bool kMasked = decltype(masked)::value;
+          auto gone = [&](int h) { return kMasked && h > 0 && h * 32 >= most; };
+          if (kMasked) {
+            const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
+#pragma unroll
+            for (int h = 0; h < kKeys / 32; ++h)
+              if (!gone(h) && least < h * 32 + 32) {
+#pragma unroll
+                for (int i = h * 32; i < h * 32 + 32; ++i)
+                  if (i >= seen) x[i] = -INFINITY;
+              }
+          }
+          // The first piece goes ahead with the maximum so far (an item's first
+          // tile: with the piece's own), while the tile's is found; rarely, it
+          // has to be done again.
+          auto max_of = [&](int h, float m) {
+            float m2 = fmaxf(x[h * 32], x[h * 32 + 1]);
+#pragma unroll
+            for (int i = h * 32 + 2; i < h * 32 + 30; i += 4) {
+              m = max3(m, x[i], x[i + 1]);
+              m2 = max3(m2, x[i + 2], x[i + 3]);
+            }
+            return max3(m, m2, fmaxf(x[h * 32 + 30], x[h * 32 + 31]));
+          };
+          float m_tile = max_of(0, kFloor);
+          if (j == 0) m_used = m_tile;
           uint32_t w[16];
-          float mx[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(x[e], x[4 + e]);
-#pragma unroll
-          for (int i = 8; i < kKeys; i += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[i + 2 * e], x[i + 2 * e + 1]);
           piece(x, w);
-          const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+#pragma unroll
+          for (int h = 1; h < kKeys / 32; ++h)
+            if (!gone(h)) m_tile = max_of(h, m_tile);
           if (__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag)) {
-            move_max(m_tile);
+            if (j > 0)
+              move_max(m_tile);
+            else
+              m_used = m_tile;
             sum = make_float2(0.f, 0.f);
             piece(x, w);
           }
           store(0, w);
 #pragma unroll
           for (int h = 1; h < kKeys / 32; ++h) {
-            piece(x + h * 32, w);
-            store(h, w);
-          }
-        } else {
-          // The first tile, or one that some row does not see whole.
-          const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
-          const int32_t most = t0 + warp_tok1 + 1 - j * kKeys;  // and that any row of the warp does
-          float m_tile = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < kKeys / 32; ++h) {
-            if (h * 32 >= most) continue;
-            if (least < h * 32 + 32) {
-#pragma unroll
-              for (int i = h * 32; i < h * 32 + 32; ++i)
-                if (i >= seen) x[i] = -INFINITY;
-            }
-            float m2 = m_tile;
-#pragma unroll
-            for (int i = h * 32; i < h * 32 + 32; i += 4) {
-              m_tile = max3(m_tile, x[i], x[i + 1]);
-              m2 = max3(m2, x[i + 2], x[i + 3]);
-            }
-            m_tile = fmaxf(m_tile, m2);
-          }
-          if (j == 0)
-            m_used = fmaxf(m_tile, kFloor);
-          else if (__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag))
-            move_max(m_tile);
-#pragma unroll
-          for (int h = 0; h < kKeys / 32; ++h) {
-            uint32_t w[16];
-            if (h * 32 < most) {
-              piece(x + h * 32, w);
-            } else {
+            if (gone(h)) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) w[i] = 0u;
+            } else {
+              piece(x + h * 32, w);
             }
             store(h, w);
           }
-        }
+        };
+        if (least >= kKeys)
+          tile(std::integral_constant<bool, false>{});
+        else
+          tile(std::integral_constant<bool, true>{});
         l += sum.x + sum.y;
       }
       // The sums go to the output warps, by two slots (and barriers) in turn: the
