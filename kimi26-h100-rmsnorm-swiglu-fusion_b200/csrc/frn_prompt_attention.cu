@@ -833,19 +833,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int warp_tok0 = (warp & 3) * 32 / p.group;  // token of the warp's first row
     const uint32_t stage = smem_addr(smem + C::OFF_OUT) + (warp & 3) * (C::NOUT * 2048);
-    uint32_t no[2] = {0, 0};  // items so far
+    uint32_t no0 = 0, no1 = 0;  // items so far, of each row tile
     bool ok = true;
     PromptItem item;
     for (int32_t it = 0; ok && next_item(it, item); ++it) {
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < 2; ++s) {
         if (tiles_of(item, s) == 0) continue;
+        const uint32_t done = s ? no1 : no0;
         const int32_t tok = item.t0 + s * p.tq + row_tok;
         const uint32_t tm_o = tmem + lanes + C::TM_O + s * DV;
-        const uint32_t slot = no[s] & 1u;
-        ok = ok && mbar_wait(&l_full[slot * 2 + s], (no[s] >> 1) & 1u, abort_flag, to) &&
-             mbar_wait(&o_full[s], no[s] & 1u, abort_flag, to);
-        ++no[s];
+        const uint32_t slot = done & 1u;
+        ok = ok && mbar_wait(&l_full[slot * 2 + s], (done >> 1) & 1u, abort_flag, to) &&
+             mbar_wait(&o_full[s], slot, abort_flag, to);
+        if (s) ++no1; else ++no0;
         if (!ok) break;
         tc_fence_after();
         const float inv =
@@ -1005,62 +1006,54 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         };
         const int32_t least = t0 + warp_tok0 + 1 - j * kKeys;  // keys that every row sees
         const int32_t most = t0 + warp_tok1 + 1 - j * kKeys;   // and that any row does
-        auto tile = [&](auto masked) {
-          constexpr bool kMasked = decltype(masked)::value;
-          auto gone = [&](int h) { return kMasked && h > 0 && h * 32 >= most; };
-          if (kMasked) {
-            const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
+        if (least < kKeys) {
+          const int32_t seen = tok + 1 - j * kKeys;  // keys of this tile that the row sees
 #pragma unroll
-            for (int h = 0; h < kKeys / 32; ++h)
-              if (!gone(h) && least < h * 32 + 32) {
+          for (int h = 0; h < kKeys / 32; ++h)
+            if (least < h * 32 + 32) {
 #pragma unroll
-                for (int i = h * 32; i < h * 32 + 32; ++i)
-                  if (i >= seen) x[i] = -INFINITY;
-              }
-          }
-          // The first piece goes ahead with the maximum so far (an item's first
-          // tile: with the piece's own), while the tile's is found; rarely, it
-          // has to be done again.
-          auto max_of = [&](int h, float m) {
-            float m2 = fmaxf(x[h * 32], x[h * 32 + 1]);
-#pragma unroll
-            for (int i = h * 32 + 2; i < h * 32 + 30; i += 4) {
-              m = max3(m, x[i], x[i + 1]);
-              m2 = max3(m2, x[i + 2], x[i + 3]);
+              for (int i = h * 32; i < h * 32 + 32; ++i)
+                if (i >= seen) x[i] = -INFINITY;
             }
-            return max3(m, m2, fmaxf(x[h * 32 + 30], x[h * 32 + 31]));
-          };
-          float m_tile = max_of(0, kFloor);
-          if (j == 0) m_used = m_tile;
-          uint32_t w[16];
+        }
+        auto max_of = [&](int h, float m) {
+          float m2 = fmaxf(x[h * 32], x[h * 32 + 1]);
+#pragma unroll
+          for (int i = h * 32 + 2; i < h * 32 + 30; i += 4) {
+            m = max3(m, x[i], x[i + 1]);
+            m2 = max3(m2, x[i + 2], x[i + 3]);
+          }
+          return max3(m, m2, fmaxf(x[h * 32 + 30], x[h * 32 + 31]));
+        };
+        // The first piece goes ahead with the maximum so far (an item's first
+        // tile: with the piece's own), while the tile's is found; rarely, it has
+        // to be done again.
+        float m_tile = max_of(0, kFloor);
+        if (j == 0) m_used = m_tile;
+        uint32_t w[16];
+#pragma unroll 1
+        for (;;) {
           piece(x, w);
 #pragma unroll
-          for (int h = 1; h < kKeys / 32; ++h)
-            if (!gone(h)) m_tile = max_of(h, m_tile);
-          if (__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag)) {
-            if (j > 0)
-              move_max(m_tile);
-            else
-              m_used = m_tile;
-            sum = make_float2(0.f, 0.f);
-            piece(x, w);
-          }
-          store(0, w);
+          for (int h = 1; h < kKeys / 32; ++h) m_tile = max_of(h, m_tile);
+          if (!__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag)) break;
+          if (j > 0)
+            move_max(m_tile);
+          else
+            m_used = fmaxf(m_used, m_tile);
+          sum = make_float2(0.f, 0.f);
+        }
+        store(0, w);
 #pragma unroll
-          for (int h = 1; h < kKeys / 32; ++h) {
-            if (gone(h)) {
+        for (int h = 1; h < kKeys / 32; ++h) {
+          if (h * 32 < most) {
+            piece(x + h * 32, w);
+          } else {  // no row of the warp sees these keys
 #pragma unroll
-              for (int i = 0; i < 16; ++i) w[i] = 0u;
-            } else {
-              piece(x + h * 32, w);
-            }
-            store(h, w);
+            for (int i = 0; i < 16; ++i) w[i] = 0u;
           }
-        };
-        if (least >= kKeys)
-          tile(std::integral_constant<bool, false>{});
-        else
-          tile(std::integral_constant<bool, true>{});
+          store(h, w);
+        }
         l += sum.x + sum.y;
       }
       // The sums go to the output warps, by two slots (and barriers) in turn: the
