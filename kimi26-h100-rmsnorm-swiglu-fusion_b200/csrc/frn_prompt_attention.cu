@@ -986,12 +986,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             if (lane == 0) mbar_arrive(h == kKeys / 32 - 1 ? &p_ready[s] : &p_most[s]);
           }
         };
-        // A new maximum for the rows: what was summed so far is brought to it.
-        auto move_max = [&](float m_tile) {
+        // A new maximum for the rows that need one: what was summed so far is
+        // brought to it.  The others keep theirs (their factor is one): a row's
+        // bits must not depend on what lies in the rows beside it.
+        auto move_max = [&](float m_new) {
           // PV(j - 1) is complete (see the order of issue) and PV(j) waits for
           // this P, so O is this warp's to change.
-          const float m_new = fmaxf(m_used, m_tile);
-          const float c = prompt_exp2((m_used - m_new) * p.qscale);
+          const float c = m_new == m_used ? 1.f : prompt_exp2((m_used - m_new) * p.qscale);
           m_used = m_new;
           l *= c;
 #pragma unroll
@@ -1036,11 +1037,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           piece(x, w);
 #pragma unroll
           for (int h = 1; h < kKeys / 32; ++h) m_tile = max_of(h, m_tile);
-          if (!__any_sync(0xffffffffu, (m_tile - m_used) * p.qscale > kLag)) break;
+          const bool grow = (m_tile - m_used) * p.qscale > kLag;
+          if (!__any_sync(0xffffffffu, grow)) break;
+          const float m_new = grow ? m_tile : m_used;
           if (j > 0)
-            move_max(m_tile);
+            move_max(m_new);
           else
-            m_used = fmaxf(m_used, m_tile);
+            m_used = m_new;
           sum = make_float2(0.f, 0.f);
         }
         store(0, w);

@@ -197,6 +197,25 @@ def test_nothing_to_do():
     assert run(q[:0], k[:0], v[:0], [0, 0], 0.1, longest=0).shape == (0, 4, 128)
 
 
+@pytest.mark.parametrize("heads", [(7, 1, 64, 64), (5, 1, 128, 128), (3, 1, 192, 128)],
+                         ids=lambda x: "x".join(map(str, x)))
+def test_bits_do_not_depend_on_the_neighbourhood(heads):
+    """A row's bits are the same whatever ran on the SM before and whatever lies
+    beside it (rows of no token take part in the tiles): with large values, so
+    that maxima move."""
+    lens = [77, 130, 9]
+    q, k, v, cu = make(lens, *heads, dtype=torch.float16, seed=21)
+    q = q * 6
+    alone = [run(q[a:b], k[a:b], v[a:b], [0, b - a], 0.3) for a, b in zip(cu[:-1], cu[1:])]
+    for noise in (0.0, 100.0, -100.0):
+        other = torch.full((400, *q.shape[1:]), noise, dtype=q.dtype)
+        run(other, torch.ones(400, *k.shape[1:], dtype=k.dtype),
+            torch.ones(400, *v.shape[1:], dtype=v.dtype), [0, 400], 0.3)
+        got = run(q, k, v, cu, 0.3)
+        for a, b, one in zip(cu[:-1], cu[1:], alone):
+            assert torch.equal(got[a:b], one)
+
+
 def test_streams_graphs_and_repeats():
     q, k, v, cu = make([200, 333], 8, 2, 128, 128, seed=8)
     first = run(q, k, v, cu, 0.09)
