@@ -965,7 +965,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         // exp2 of 32 scores, their P and their sum.
         auto piece = [&](const float* v, uint32_t (&w)[16]) {
           const float2 scale2 = make_float2(p.qscale, p.qscale);
-          const float2 shift2 = make_float2(-m_used * p.qscale, -m_used * p.qscale);
+          // fp16: P is kept 2^7 higher (it stays below 2^15), so that fewer small
+          // ones fall below the type's normal range; the sums carry the same factor.
+          constexpr float kUp = Elem16<T>::kUmmaFormat == 0u ? 15.f - kLag : 0.f;
+          const float shift = fmaf(-m_used, p.qscale, kUp);
+          const float2 shift2 = make_float2(shift, shift);
           float2 part[2];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
