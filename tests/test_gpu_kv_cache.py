@@ -134,6 +134,23 @@ def test_pages_copy_many_pairs():
     assert all(torch.equal(p, w) for p, w in zip(pools, want))
 
 
+def test_offsets_past_32_bits():
+    """Pools of more than 2^32 elements: tokens appended to the last page, the page copied."""
+    P, page, Hkv, D = 4200, 1024, 8, 128
+    pools = [torch.zeros(P, page, Hkv, D, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    assert pools[0].numel() > 2 ** 32
+    k, v = (t.to(DEV) for t in new_tokens(5, Hkv, D, torch.bfloat16, 9))
+    table = torch.tensor([[0, P - 1]], dtype=torch.int32, device=DEV)
+    start = torch.tensor([2 * page - 5], dtype=torch.int32, device=DEV)
+    capi.kv_cache_append(k, v, *pools, table, start, torch.tensor([0, 5]).int().to(DEV))
+    capi.kv_pages_copy(pools, [P - 1, P - 1], [P - 3, 1])
+    for pool, new in zip(pools, (k, v)):
+        for at in (P - 1, P - 3, 1):
+            assert torch.equal(pool[at, page - 5:], new) and (pool[at, :page - 5] == 0).all()
+        assert (pool[P - 2] == 0).all() and (pool[0] == 0).all()
+    assert capi.device_error(0) == 0
+
+
 def test_pages_copy_surface():
     from src.load_gqa_attention import gqa_attention_cuda as ops
 

@@ -164,6 +164,24 @@ def test_strided_views():
     orc.assert_close(run(q, k, kv.to(DEV)[..., 128:], cu, 0.07), ref, spread)
 
 
+def test_offsets_past_32_bits():
+    """More than 2^32 elements of q and out; the first and the last sequence are looked at."""
+    n, count, Hq, Hkv, D = 100, 2700, 128, 8, 128
+    q = torch.zeros(n * count, Hq, D, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(n * count, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros(n * count, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    assert q.numel() > 2 ** 32
+    q1, k1, v1, _ = make([n], Hq, Hkv, D, D, seed=13)
+    for rows in (slice(0, n), slice(n * (count - 1), None)):
+        q[rows], k[rows], v[rows] = q1.to(DEV), k1.to(DEV), v1.to(DEV)
+    cu = torch.arange(count + 1, dtype=torch.int32, device=DEV) * n
+    got = capi.gqa_prompt_attention(q, k, v, cu, n, 0.1)
+    ref, spread = orc.prompt_attention(q1, k1, v1, [0, n], 0.1)
+    orc.assert_close(got[:n], ref, spread)
+    orc.assert_close(got[-n:], ref, spread)
+    assert (got[n:2 * n] == 0).all() and capi.device_error(0) == 0
+
+
 def test_rows_of_no_sequence_are_left_alone():
     q, k, v, _ = make([90], 4, 2, 128, 128, seed=5)
     cu = [10, 40, 80]
@@ -236,6 +254,28 @@ def test_streams_graphs_and_repeats():
     torch.cuda.synchronize()
     ref, spread = orc.prompt_attention(qd.cpu(), k, v, cu, 0.09)
     orc.assert_close(out, ref, spread)
+
+
+def test_beside_other_work():
+    """Bits and answers are the same while another stream keeps the SMs busy."""
+    lens = [77, 300, 1, 160]
+    q, k, v, cu = (t.to(DEV) if torch.is_tensor(t) else t for t in make(lens, 7, 1, 64, 64, seed=4))
+    cud = torch.tensor(cu, dtype=torch.int32, device=DEV)
+    busy = [t.to(DEV) for t in make([700] * 8, 16, 4, 128, 128, seed=5)[:3]]
+    busy_cu = torch.arange(9, dtype=torch.int32, device=DEV) * 700
+    first = capi.gqa_prompt_attention(q, k, v, cud, 300, 0.1)
+    busy_first = capi.gqa_prompt_attention(*busy, busy_cu, 700, 0.1)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    got, busy_got = [], []
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            busy_got.append(capi.gqa_prompt_attention(*busy, busy_cu, 700, 0.1))
+        got.append(capi.gqa_prompt_attention(q, k, v, cud, 300, 0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, first) for x in got)
+    assert all(torch.equal(x, busy_first) for x in busy_got)
+    assert capi.device_error(0) == 0
 
 
 def test_python_surface():
