@@ -31,8 +31,8 @@
 // What bounds it: HBM.  8 sequences of 100 to 131 thousand tokens (3.8 GB) take
 // 596 to 631 us, 6.0 to 6.4 TB/s or 92 to 98% of a plain copy's rate; 64 sequences
 // of 1 to 8192 tokens (352 MB) 67 to 70 us, about 10 of them the start of the
-// streams and the join; one sequence of 1000 tokens 8.8 us, of which an empty
-// call's chain of dependent loads and two launches is 5.6.  Two CTAs an SM with
+// streams and the join; one sequence of 1000 tokens 8.5 us, of which a one-token
+// call's chain of dependent loads and two launches is 5.7.  Two CTAs an SM with
 // three tiles in flight a warp: one CTA with seven is 6 to 20% slower, three with
 // two up to 12%.
 //
@@ -42,7 +42,10 @@
 // type for the second product, its row sums are not (a second product with what
 // the rounding leaves would take the error from 1.4 times the output's own
 // rounding to that, and costs 2 to 4% of the time).  fp32: CUDA cores, one
-// token a lane for the scores, head dims across lanes for the output.
+// token a lane for the scores, head dims across lanes for the output.  Four heads'
+// scores are taken together, so that their shuffles and exponentials overlap: 8
+// sequences of 8192 tokens, 32 / 8 heads of 128, take 132 us instead of 158 (4.1
+// TB/s; four warps an SM leave the latencies of shared memory uncovered).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -257,6 +260,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
   constexpr int NR = MMA ? (GMAX + 7) / 8 : 1;  // 8-row halves of the MMA in use
   constexpr int NKC = D / 16, NDT = D / 8;
   constexpr int E = D / 32;                     // fp32: output dims of a lane
+  constexpr int HB = GMAX > 4 ? 4 : 1;          // fp32: heads whose scores are taken together
   constexpr int CHUNKS = C::ROW_BYTES / 16;     // 16-byte pieces of a row
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ int64_t sm_warp[kPagedWarps];
@@ -309,7 +313,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
 
   uint8_t* ring = smem + warp * C::WARP_BYTES;
   const uint32_t ring_a = smem_addr(ring);
-  float* sm_q = reinterpret_cast<float*>(ring + C::RING_BYTES);  // fp32: [G][D]
+  float* sm_q = reinterpret_cast<float*>(ring + C::RING_BYTES);  // fp32: [GMAX][D]
 
   // ---- loads: the page of a tile (or of each of its tokens, one a lane) is
   // looked up one tile before the tile's copies are issued.
@@ -418,8 +422,16 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
         }
       } else {
         __syncwarp();  // every lane is done with the last item's queries
-        for (int i = lane; i < G * D; i += 32)
-          sm_q[i] = static_cast<float>(qp[(i / D) * p.q_head + i % D]);
+        float qv[GMAX][E];
+#pragma unroll
+        for (int r = 0; r < GMAX; ++r)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            qv[r][e] = r < G ? static_cast<float>(qp[r * p.q_head + e * 32 + lane]) : 0.f;
+#pragma unroll
+        for (int r = 0; r < GMAX; ++r)
+#pragma unroll
+          for (int e = 0; e < E; ++e) sm_q[r * D + e * 32 + lane] = qv[r][e];
         __syncwarp();
 #pragma unroll
         for (int r = 0; r < GMAX; ++r) {
@@ -498,32 +510,55 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
       __syncwarp();  // K is read: its place takes the probabilities, [token][head]
       float s[GMAX];
 #pragma unroll
-      for (int r = 0; r < GMAX; ++r) {
-        s[r] = 0.f;
-        if (r >= G) continue;
-        const float4* qf = reinterpret_cast<const float4*>(sm_q + r * D) + half * (CHUNKS / 2);
-        float2 d0 = make_float2(0.f, 0.f), d1 = d0;
+      for (int r4 = 0; r4 < GMAX; r4 += HB) {
+        if (r4 >= G) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS / 2; ++c) {
-          const float4 q4 = qf[c];
-          d0 = fma_f32x2(make_float2(q4.x, q4.y), make_float2(kf[c].x, kf[c].y), d0);
-          d1 = fma_f32x2(make_float2(q4.z, q4.w), make_float2(kf[c].z, kf[c].w), d1);
+          for (int r = 0; r < HB; ++r) s[r4 + r] = 0.f;
+          continue;
         }
-        float x = (d0.x + d0.y) + (d1.x + d1.y);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        float bm = live ? x * p.qscale : -FLT_MAX;
+        float x[HB], bm[HB];
 #pragma unroll
-        for (int w = 8; w > 0; w >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, w));
-        const float m_new = fmaxf(m_run[r], bm);  // the same in every lane
-        if (m_new != m_run[r]) {
-          const float corr = exp2f(m_run[r] - m_new);
-          m_run[r] = m_new;
-          l_run[r] *= corr;
+        for (int r = 0; r < HB; ++r) {
+          const float4* qf =
+              reinterpret_cast<const float4*>(sm_q + (r4 + r) * D) + half * (CHUNKS / 2);
+          float2 d0 = make_float2(0.f, 0.f), d1 = d0;
 #pragma unroll
-          for (int e = 0; e < E; ++e) accf[r][e] *= corr;
+          for (int c = 0; c < CHUNKS / 2; ++c) {
+            const float4 q4 = qf[c];
+            d0 = fma_f32x2(make_float2(q4.x, q4.y), make_float2(kf[c].x, kf[c].y), d0);
+            d1 = fma_f32x2(make_float2(q4.z, q4.w), make_float2(kf[c].z, kf[c].w), d1);
+          }
+          x[r] = (d0.x + d0.y) + (d1.x + d1.y);
         }
-        s[r] = live ? exp2f(fmaf(x, p.qscale, -m_new)) : 0.f;
-        l_run[r] += half == 0 ? s[r] : 0.f;  // one of the two copies counts
+#pragma unroll
+        for (int r = 0; r < HB; ++r) x[r] += __shfl_xor_sync(0xffffffffu, x[r], 16);
+#pragma unroll
+        for (int r = 0; r < HB; ++r) bm[r] = live ? x[r] * p.qscale : -FLT_MAX;
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+          for (int r = 0; r < HB; ++r)
+            bm[r] = fmaxf(bm[r], __shfl_xor_sync(0xffffffffu, bm[r], w));
+        // The maxima are the same in every lane.
+        bool grows = false;
+#pragma unroll
+        for (int r = 0; r < HB; ++r) grows |= bm[r] > m_run[r4 + r];
+        if (grows) {
+#pragma unroll
+          for (int r = 0; r < HB; ++r) {
+            const float m_new = fmaxf(m_run[r4 + r], bm[r]);
+            const float corr = exp2f(m_run[r4 + r] - m_new);
+            m_run[r4 + r] = m_new;
+            l_run[r4 + r] *= corr;
+#pragma unroll
+            for (int e = 0; e < E; ++e) accf[r4 + r][e] *= corr;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < HB; ++r) {
+          s[r4 + r] = live ? exp2f(fmaf(x[r], p.qscale, -m_run[r4 + r])) : 0.f;
+          l_run[r4 + r] += half == 0 ? s[r4 + r] : 0.f;  // one of the two copies counts
+        }
       }
       if (half == 0) {
 #pragma unroll
@@ -625,13 +660,11 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
 }
 
 // Sum of the parts s0, s0 + step, ... of one row, brought to their largest
-// maximum; a lane holds D / 32 dims.  The loads of the parts do not depend on one
-// another.
-template <int E>
+// maximum; a lane holds D / 32 dims.  The loads of U parts do not depend on one another.
+template <int E, int U>
 __device__ __forceinline__ void join_parts(const PagedDecodeParams& p, const float* mls, int first,
                                            int w0, int n, int s0, int step, int row, int lane,
                                            float (&acc)[E], float& mx, float& den) {
-  constexpr int U = 4;
   mx = -FLT_MAX;
   den = 0.f;
 #pragma unroll
@@ -672,13 +705,13 @@ __device__ __forceinline__ void join_parts(const PagedDecodeParams& p, const flo
 // Joins the parts of every item that was cut, in share order, and writes the
 // zeros of empty sequences.  A CTA has join_rows query heads of one KV head:
 // four where there are many rows (and so few parts of each), a warp each; one
-// where there are few.  An item of many parts is joined by the four warps
-// together, row by row.
-template <typename T, int D>
-__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDecodeParams p) {
+// where there are few.  An item of many parts is joined by the W warps together,
+// row by row.
+template <typename T, int D, int W, int U>  // W warps, U parts at once
+__global__ void __launch_bounds__(32 * W) paged_join_kernel(const PagedDecodeParams p) {
   constexpr int E = D / 32;
-  __shared__ float sm_acc[kPagedWarps][D];
-  __shared__ float2 sm_ml[kPagedWarps];
+  __shared__ float sm_acc[W][D];
+  __shared__ float2 sm_ml[W];
   griddep_launch_dependents();
   griddep_wait();
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
@@ -691,7 +724,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDe
   const int2 join =
       *reinterpret_cast<const int2*>(p.joins + (static_cast<int64_t>(b) * p.hkv + head) * 2);
   if (p.seq_lens[b] <= 0 || p.kv.max_pages == 0) {
-    for (int i = static_cast<int>(threadIdx.x); i < rows * D; i += kPagedThreads)
+    for (int i = static_cast<int>(threadIdx.x); i < rows * D; i += 32 * W)
       op[(i / D) * p.out_head + i % D] = from_float<T>(0.f);
     return;
   }
@@ -701,7 +734,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDe
   float acc[E], mx, den;
   if (rows > 1 && n <= 16) {
     if (warp < rows) {
-      join_parts<E>(p, mls, join.x, w0, n, 0, 1, row0 + warp, lane, acc, mx, den);
+      join_parts<E, U>(p, mls, join.x, w0, n, 0, 1, row0 + warp, lane, acc, mx, den);
 #pragma unroll
       for (int e = 0; e < E; ++e)
         op[warp * p.out_head + lane * E + e] = from_float<T>(acc[e] / den);
@@ -709,19 +742,19 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedDe
     return;
   }
   for (int r = 0; r < rows; ++r) {
-    join_parts<E>(p, mls, join.x, w0, n, warp, kPagedWarps, row0 + r, lane, acc, mx, den);
+    join_parts<E, U>(p, mls, join.x, w0, n, warp, W, row0 + r, lane, acc, mx, den);
     if (r > 0) __syncthreads();  // the last row's meeting is over
 #pragma unroll
     for (int e = 0; e < E; ++e) sm_acc[warp][lane * E + e] = acc[e];
     if (lane == 0) sm_ml[warp] = make_float2(mx, den);
     __syncthreads();
-    for (int d = static_cast<int>(threadIdx.x); d < D; d += kPagedThreads) {
+    for (int d = static_cast<int>(threadIdx.x); d < D; d += 32 * W) {
       float m = -FLT_MAX;
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) m = fmaxf(m, sm_ml[w].x);
+      for (int w = 0; w < W; ++w) m = fmaxf(m, sm_ml[w].x);
       float num = 0.f, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kPagedWarps; ++w) {
+      for (int w = 0; w < W; ++w) {
         const float f = exp2f(sm_ml[w].x - m);
         num = fmaf(sm_acc[w][d], f, num);
         sum = fmaf(sm_ml[w].y, f, sum);
@@ -788,13 +821,31 @@ static int launch_paged(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaS
       static_cast<unsigned>(p.hkv * ((p.group + p.join_rows - 1) / p.join_rows)),
       static_cast<unsigned>(g.batch));
   cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, p);
+  // Few rows: twice the parts of a row at once, and from 64 parts on twice the warps
+  // (32 / 8 heads of 128, one sequence of 1000 tokens, cold, 32 parts: 9.5 us with
+  // the first, 10.3 with both, 9.8 with neither; of 4000, 125 parts: 11.9, 10.3,
+  // 13.8; a batch of 64 sequences loses 1 us by either).
+  const int64_t parts = g.kv.max_pages * g.kv.page_size / (kTileTokens * p.least_share);
+  const bool few = g.batch * g.num_q_heads < sm_count(dev) / 2;
+  if (few && parts > 64) {
+    cfg.blockDim = dim3(2 * kPagedThreads);
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, 2 * kPagedWarps, 8>, p);
+  } else if (few && parts > 16) {
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, kPagedWarps, 8>, p);
+  } else {
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D, kPagedWarps, 4>, p);
+  }
   if (e != cudaSuccess) return set_cuda_error("launch paged_join", e);
   return 0;
 }
 
 template <typename T, int D>
 static int launch_paged_g(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaStream_t s) {
+  // fp32: one or two heads, one after the other, where four together would be
+  // mostly padding (8 sequences of 8192 tokens, 8 heads of their own: 122 us
+  // instead of 130).
+  if constexpr (sizeof(T) == 4)
+    if (p.group <= 2) return launch_paged<T, D, 4>(g, p, s);
   return p.group <= 8 ? launch_paged<T, D, 8>(g, p, s) : launch_paged<T, D, 16>(g, p, s);
 }
 
