@@ -41,14 +41,17 @@
 // for the second product; the row sums are of the unrounded values, in fp32.
 //
 // What bounds it.  Of a K/V tile and both row tiles the tensor core has 2048
-// clocks of work (D = 128), the special-function units 2048; a round takes 2840:
-// the way of one row tile from a finished S through its exponentials (1800), the
-// rest of PV and the next S (750) and two barriers (300).  One prompt of 8192
-// tokens, 32 / 8 heads of 128, bf16: 430 us (1270 TFLOP/s) in short runs at
-// 1.73 GHz, 490 to 510 us (1100 TFLOP/s) without pause, where the power limit
-// holds the clock at 1.49 GHz; MLA heads (192 / 128) 720 TFLOP/s, 24 packed
-// prompts of 16 to 1500 tokens 640 TFLOP/s (items of one to twelve tiles: the
-// first tile's maximum cannot be guessed, and both row tiles begin together).
+// clocks of work (D = 128), the special-function units 2048; a round takes about
+// 2600: the way of one row tile from a finished S through its exponentials, the
+// rest of PV and the next S, and two barriers.  One prompt of 8192 tokens, 32 / 8
+// heads of 128, bf16: 401 to 417 us (1320 to 1370 TFLOP/s) in short runs at 1.73
+// GHz, 469 to 490 us (1120 to 1170 TFLOP/s) without pause, where the power limit
+// holds the clock at 1.49 GHz; MLA heads (192 / 128) of 500 to 2048 tokens 240 us
+// (790 TFLOP/s; 13% of the products are masked parts of diagonal tiles), 24 packed
+// prompts of 16 to 1500 tokens 97 to 99 us (680 TFLOP/s; items of one to twelve
+// tiles: the first tile's maximum cannot be guessed).  The instructions of a round
+// should stay in cache: one copy of the tile code for whole and masked tiles, 16 KB
+// less, took 500 us to 485.
 // Not adopted: a quarter or half of the exponentials by polynomial (no gain once
 // the registers sufficed, 2.5% at D = 64), two threads a row (the maximum has to
 // be agreed on: 611 us), spinning instead of suspended waits (3% slower).
@@ -87,7 +90,7 @@ struct PromptCfg {
   // Keys of a K/V tile.  With 192 columns 96 of them, so that K and V tiles fit
   // twice beside the two Q tiles (with 128 a second V tile does not, and every
   // tile waits for its V: 308 us for four sequences of 500 to 2048 tokens, 64
-  // heads, 289 with 96; with 64 a product takes 48 clocks of the tensor core where
+  // heads, 289 with 96, both before the later steps; with 64 a product takes 48 clocks of the tensor core where
   // 32 would do, for its operands' shared-memory reads).
   static constexpr int KEYS = DQK == 192 ? 96 : 128;
   static constexpr int MOST = KEYS - 32;             // keys whose P is announced before the rest
@@ -247,7 +250,8 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
 // True in one lane of a converged warp.  Unlike a test of the lane number this
 // tells the compiler that the branch is for a single thread, so that the MMA's
 // uniform operands need no loop over lanes: the eight MMAs of a PV are issued in
-// 450 clocks instead of 770, the whole of 8192 tokens takes 586 us instead of 669.
+// 450 clocks instead of 770 (8192 tokens, without the later steps: 586 us instead of
+// 669).
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
   asm volatile(
