@@ -90,8 +90,9 @@ struct PromptCfg {
   // Keys of a K/V tile.  With 192 columns 96 of them, so that K and V tiles fit
   // twice beside the two Q tiles (with 128 a second V tile does not, and every
   // tile waits for its V: 308 us for four sequences of 500 to 2048 tokens, 64
-  // heads, 289 with 96, both before the later steps; with 64 a product takes 48 clocks of the tensor core where
-  // 32 would do, for its operands' shared-memory reads).
+  // heads, 289 with 96, both before the later steps; with 64 a product takes 48
+  // clocks of the tensor core where 32 would do, for its operands' shared-memory
+  // reads).
   static constexpr int KEYS = DQK == 192 ? 96 : 128;
   static constexpr int MOST = KEYS - 32;             // keys whose P is announced before the rest
   static constexpr int QHALF = kRows * 128;          // bytes of 128 rows x 64 columns
