@@ -235,6 +235,15 @@ __device__ __forceinline__ void reg_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// All N columns of this lane's row of scores: as many as `x` has room for.
+template <int N>
+__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, float (&x)[N]) {
+  static_assert(N % 32 == 0, "whole loads of 32 columns");
+#pragma unroll
+  for (int c = 0; c < N / 32; ++c)
+    tmem_ld_32x32b_x32(taddr + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c * 32]));
+}
+
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -962,9 +971,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!ok) break;
         tc_fence_after();
         float x[kKeys];
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld_32x32b_x32(tm_s + c * 32, reinterpret_cast<uint32_t(&)[32]>(x[c * 32]));
+        tmem_ld_row(tm_s, x);
         tmem_ld_wait();
         float2 sum = make_float2(0.f, 0.f);
         // exp2 of 32 scores, their P and their sum.
