@@ -66,6 +66,7 @@
 
 #include "frn_internal.h"
 #include "frn_ptx.cuh"
+#include "frn_take_over.h"
 
 namespace frn {
 
@@ -588,7 +589,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       // Blocks of all sequences, for one head.  Items are fewer than 2^31: their
       // numbers are those of CTAs.
       const int32_t blocks = finder.count(p, 0);
-      const int32_t per_group = max(1, blocks * p.heads_at_once);
+      const int64_t items_of_call = static_cast<int64_t>(blocks) * p.hkv;
+      const int32_t per_group = static_cast<int32_t>(
+          min(static_cast<int64_t>(blocks) * p.heads_at_once, static_cast<int64_t>(0x7fffffff)));
       int32_t last_group = -1;
       uint32_t answers = 0;
       auto ask = [&]() {
@@ -606,29 +609,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         index = static_cast<int32_t>(cta);
         return got;
       };
+      // The item of a number, if it has one: the grid is an upper bound.
+      auto item_of = [&](int32_t index, PromptItem& item) {
+        if (index >= items_of_call) return false;
+        const int32_t group = index / per_group;
+        const int32_t head0 = group * p.heads_at_once;
+        const int32_t heads = min(p.heads_at_once, p.hkv - head0);
+        if (group != last_group) finder.below = finder.most(p);
+        last_group = group;
+        index -= group * per_group;
+        const int32_t block = index / heads;
+        item.kvh = head0 + index - block * heads;
+        return finder.find(p, block, item);
+      };
       auto publish = [&](int32_t it) {
         if (done || !ok) return;
-        int32_t index = static_cast<int32_t>(blockIdx.x);
-        bool some = it == 0 || hear(index);
-        if (!ok) return;
-        const bool more = some;
-        if (more) ask();
         PromptItem item;
-        if (some) {
-          const int32_t group = index / per_group;
-          const int32_t head0 = group * p.heads_at_once;
-          const int32_t heads = min(p.heads_at_once, p.hkv - head0);
-          if (group != last_group) finder.below = finder.most(p);
-          last_group = group;
-          index -= group * per_group;
-          const int32_t block = heads > 0 ? index / heads : 0;
-          some = heads > 0 && blocks > 0 && finder.find(p, block, item);
-          item.kvh = head0 + index - block * heads;
-        }
-        done = !some;
+        done = !next_number(it == 0, static_cast<int32_t>(blockIdx.x), ask, hear,
+                            [&](int32_t index) { return item_of(index, item); });
+        if (!ok) return;
         if (done) item.len = 0;  // the end
-        if (done && more)  // numbers beyond the last item: none is left to be launched
-          while (hear(index)) ask();
         const int slot = it % kItemSlots;
         ok = ok && mbar_wait(&i_empty[slot], (static_cast<uint32_t>(it / kItemSlots) & 1u) ^ 1u,
                              abort_flag, to);

@@ -45,7 +45,7 @@ CU_SOURCES = [
     "frn_paged_decode.cu",
     "frn_kv_cache.cu",
 ]
-HEADERS = ["frn_ptx.cuh", "frn_internal.h", "frn_pair_common.cuh"]
+HEADERS = ["frn_ptx.cuh", "frn_internal.h", "frn_pair_common.cuh", "frn_take_over.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
