@@ -128,25 +128,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-template <typename T>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                          uint32_t b1) {
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (Elem16<T>::kUmmaFormat == 1u)
-      asm volatile(
-          "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
-          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-      asm volatile(
-          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
-          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-}
-
 template <bool TRANS>
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   if constexpr (TRANS)

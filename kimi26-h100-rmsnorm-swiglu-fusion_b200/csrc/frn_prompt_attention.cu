@@ -392,50 +392,180 @@ struct ItemFinder {
   }
 };
 
-// Row `tok` of one query head by the definition, a key at a time: whole warp.
-// Only for rows whose product with V met a NaN or an infinity at a position
-// that the row does not see (zero weight times that is not zero).
+// Two 16-bit elements: their exponents, all ones in one that is not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t pair) {
+  constexpr uint32_t kExp = Elem16<T>::kUmmaFormat == 0u ? 0x7c00u : 0x7f80u;
+  return ((pair & kExp) == kExp ? 0xffffu : 0u) |
+         ((pair & (kExp << 16)) == kExp << 16 ? 0xffff0000u : 0u);
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t row_pair) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(row_pair));
+  return t;
+}
+
+// The rows of a warp whose product with V met a NaN or an infinity at a position
+// that the row does not see (zero weight times that is not zero), computed once
+// more by the warp alone: 8 rows and 64 columns of V at a time, 16 keys a step, on
+// 16x8x16 MMAs (S^T = K Q^T, O^T += V^T P^T) whose operands come straight from
+// memory (the contraction of Q and K takes the head dims in an order in which a
+// lane's are 16 bytes).  Steps whose keys not every row sees take V without such
+// values and then add those that a row does see by themselves.  `rows` are the
+// lanes whose rows hold a value that is not finite, `tok` and `head` the lane's
+// row; the warp's first row is token tok0.
+// Bound by the latency of its loads.  One NaN in V at the end of a prompt makes 128
+// rows a KV head do this: 8192 tokens, 32 / 8 heads of 128, 5.6 ms instead of 0.42;
+// 65536 tokens, 4 heads of 64 on one, 18 instead of 2.6; an infinity in the same
+// column of every token makes all rows do it, 37 ms for the first of these.  (A key
+// at a time, in one chain, it would be some 450 clocks a key and row.)  16 rows at a
+// time take more registers than the output warps have: values that all warps use
+// are spilled for it, and 77 tokens with heads of 64 take 9.4 us instead of 7.7.
 template <typename T, int DQK, int DV>
-__device__ __noinline__ void exact_row(const PromptParams& p, int32_t first, int32_t tok, int kvh,
-                                       int head, int32_t covered) {
-  constexpr int EQ = DQK / 32, EV = DV / 32;
-  const int lane = static_cast<int>(threadIdx.x & 31);
-  const T* k = static_cast<const T*>(p.k) + first * p.k_token + kvh * p.k_head;
-  const T* v = static_cast<const T*>(p.v) + first * p.v_token + kvh * p.v_head;
-  bool met = false;
-  for (int32_t j = tok + 1; j < covered; ++j)
-#pragma unroll
-    for (int e = 0; e < EV; ++e)
-      met |= !isfinite(static_cast<float>(v[j * p.v_token + lane + 32 * e]));
-  if (!__any_sync(0xffffffffu, met)) return;  // the row's own keys gave the value
-  const T* q = static_cast<const T*>(p.q) + (first + tok) * p.q_token + head * p.q_head;
-  const float qs = p.negate ? -p.qscale : p.qscale;
-  float qf[EQ], acc[EV], m = -FLT_MAX, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < EQ; ++e) qf[e] = static_cast<float>(q[lane + 32 * e]) * qs;
-#pragma unroll
-  for (int e = 0; e < EV; ++e) acc[e] = 0.f;
-  for (int32_t j = 0; j <= tok; ++j) {
-    float d = 0.f;
-#pragma unroll
-    for (int e = 0; e < EQ; ++e)
-      d = fmaf(qf[e], static_cast<float>(k[j * p.k_token + lane + 32 * e]), d);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    const float m_new = fmaxf(m, d), c = exp2f(m - m_new), w = exp2f(d - m_new);
-    m = m_new;
-    l = l * c + w;
-    bool lost = true;
-#pragma unroll
-    for (int e = 0; e < EV; ++e) {
-      acc[e] = fmaf(w, static_cast<float>(v[j * p.v_token + lane + 32 * e]), acc[e] * c);
-      lost &= isnan(acc[e]);
-    }
-    if (__all_sync(0xffffffffu, lost)) break;  // NaN everywhere stays so
+__device__ __noinline__ void redo_rows(const PromptParams& p, uint32_t rows, int32_t first,
+                                       int32_t tok0, int32_t tok, int kvh, int head,
+                                       int32_t covered, volatile uint32_t* abort_flag) {
+  const int lane = static_cast<int>(threadIdx.x & 31), g = lane >> 2, tq = lane & 3;
+  const T* k = static_cast<const T*>(p.k) + first * p.k_token + kvh * p.k_head + tq * 8;
+  const T* v0 = static_cast<const T*>(p.v) + first * p.v_token + kvh * p.v_head;
+  // The last position that the rows' products covered and that holds such a value.
+  int32_t last = -1;
+  for (int32_t i = lane; i < (covered - tok0 - 1) * (DV / 8); i += 32) {
+    const int32_t j = tok0 + 1 + i / (DV / 8);
+    const uint4 x =
+        *reinterpret_cast<const uint4*>(v0 + j * p.v_token + i % (DV / 8) * 8);
+    if (odd_halves<T>(x.x) | odd_halves<T>(x.y) | odd_halves<T>(x.z) | odd_halves<T>(x.w))
+      last = j;
   }
-  T* out = static_cast<T*>(p.out) + (first + tok) * p.out_token + head * p.out_head;
+  last = __reduce_max_sync(0xffffffffu, last);
+  rows &= __ballot_sync(0xffffffffu, tok < last);  // the others' own keys gave the value
+  const float qs = p.negate ? -p.qscale : p.qscale;
+  constexpr float kUp = Elem16<T>::kUmmaFormat == 0u ? 15.f - kLag : 0.f;
+  constexpr int NC = 2;  // 32-column pieces of V at a time
+  while (rows) {
+    // The 8 rows of a pass, the last one standing in for those that are missing: the
+    // queries of row g, and the results of rows 2 tq and 2 tq + 1.
+    const int most = __popc(rows) - 1;
+    const int src = static_cast<int>(__fns(rows, 0, min(g, most) + 1));
+    const int32_t my_row = __shfl_sync(0xffffffffu, tok, src);
+    const int my_head = __shfl_sync(0xffffffffu, head, src);
+    for (int i = 0; i < 8; ++i) rows &= rows - 1;
+    const T* q = static_cast<const T*>(p.q) + (first + my_row) * p.q_token + my_head * p.q_head + tq * 8;
+    const int32_t row[2] = {__shfl_sync(0xffffffffu, my_row, tq * 8),
+                            __shfl_sync(0xffffffffu, my_row, tq * 8 + 4)};
+    const int32_t seen_by_all = __reduce_min_sync(0xffffffffu, my_row) + 1;
+    const int32_t end = __reduce_max_sync(0xffffffffu, my_row) + 1;
+#pragma unroll 1
+    for (int c0 = 0; c0 < DV; c0 += 32 * NC) {
+      const T* v = v0 + c0 + tq * 8;
+      float acc[2 * NC][4], m[2] = {-FLT_MAX, -FLT_MAX}, l[2] = {0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < EV; ++e) out[lane + 32 * e] = static_cast<T>(acc[e] / l);
+      for (int i = 0; i < 2 * NC; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll 1
+      for (int32_t j0 = 0; j0 < end; j0 += 16) {
+        const bool masked = j0 + 16 > seen_by_all;
+        float x[4] = {0.f, 0.f, 0.f, 0.f};  // key g (0, 1), g + 8 (2, 3) of rows 2 tq (0, 2), 2 tq + 1
+        const int32_t ja = min(j0 + g, end - 1), jb = min(j0 + 8 + g, end - 1);
+#pragma unroll 2
+        for (int c = 0; c < DQK; c += 32) {
+          const uint4 qa = *reinterpret_cast<const uint4*>(q + c);
+          const uint4 ka = *reinterpret_cast<const uint4*>(k + ja * p.k_token + c);
+          const uint4 kb = *reinterpret_cast<const uint4*>(k + jb * p.k_token + c);
+          const uint32_t lo[4] = {ka.x, kb.x, ka.y, kb.y}, hi[4] = {ka.z, kb.z, ka.w, kb.w};
+          mma_16816<T>(x, lo, qa.x, qa.y);
+          mma_16816<T>(x, hi, qa.z, qa.w);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          x[r] = j0 + g <= row[r] ? x[r] * qs : -INFINITY;
+          x[r + 2] = j0 + 8 + g <= row[r] ? x[r + 2] * qs : -INFINITY;
+          float m_new = fmaxf(m[r], fmaxf(x[r], x[r + 2]));
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1)
+            m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, o));
+          const float c = exp2f(m[r] - m_new);
+          m[r] = m_new;
+          l[r] *= c;
+#pragma unroll
+          for (int i = 0; i < 2 * NC; ++i) {
+            acc[i][r] *= c;
+            acc[i][r + 2] *= c;
+          }
+          x[r] = exp2f((x[r] - m_new) + kUp);
+          x[r + 2] = exp2f((x[r + 2] - m_new) + kUp);
+          l[r] += x[r] + x[r + 2];
+        }
+        const uint32_t p0 = transpose_8x8(float2_to_pair<T>(x[0], x[1]));
+        const uint32_t p1 = transpose_8x8(float2_to_pair<T>(x[2], x[3]));
+        uint32_t odd = 0;  // of keys g (low half) and g + 8
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const uint4 va = *reinterpret_cast<const uint4*>(v + ja * p.v_token + c * 32);
+          const uint4 vb = *reinterpret_cast<const uint4*>(v + jb * p.v_token + c * 32);
+          uint32_t a[4] = {va.x, va.y, va.z, va.w}, b[4] = {vb.x, vb.y, vb.z, vb.w};
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t oa = odd_halves<T>(a[i]), ob = odd_halves<T>(b[i]);
+              odd |= (oa ? 1u : 0u) | (ob ? 2u : 0u);
+              a[i] &= ~oa;
+              b[i] &= ~ob;
+            }
+          }
+          // Rows of a product: 8 columns of each of two words.
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const uint32_t vt[4] = {transpose_8x8(a[i]), transpose_8x8(a[i + 1]),
+                                    transpose_8x8(b[i]), transpose_8x8(b[i + 1])};
+            mma_16816<T>(acc[c * 2 + i / 2], vt, p0, p1);
+          }
+        }
+        if (masked) {
+          const uint32_t lanes_a = __ballot_sync(0xffffffffu, odd & 1u);
+          const uint32_t lanes_b = __ballot_sync(0xffffffffu, odd & 2u);
+#pragma unroll 1
+          for (int t = 0; t < 16 && j0 + t < end; ++t) {
+            if (!((t < 8 ? lanes_a : lanes_b) >> ((t & 7) * 4) & 15u)) continue;
+            // The weights of key t, from the lanes that hold them.
+            const int from = (t & 7) * 4 + tq;
+            const float w0 = __shfl_sync(0xffffffffu, t < 8 ? x[0] : x[2], from);
+            const float w1 = __shfl_sync(0xffffffffu, t < 8 ? x[1] : x[3], from);
+            // Results of this lane: column (g / 2) * 8 + 2 i + g % 2 of word i.
+            const T* vr = v0 + c0 + (j0 + t) * p.v_token + (g >> 1) * 8 + (g & 1);
+#pragma unroll
+            for (int i = 0; i < 4 * NC; ++i) {
+              const float y = static_cast<float>(vr[(i / 4) * 32 + (i % 4) * 2]);
+              float* o = acc[i / 2] + (i & 1) * 2;
+              if (!isfinite(y)) {
+                if (j0 + t <= row[0]) o[0] = fmaf(w0, y, o[0]);
+                if (j0 + t <= row[1]) o[1] = fmaf(w1, y, o[1]);
+              }
+            }
+          }
+        }
+        bool lost = true;
+#pragma unroll
+        for (int i = 0; i < 2 * NC; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) lost &= isnan(acc[i][e]);
+        if (__all_sync(0xffffffffu, lost)) break;  // NaN everywhere stays so
+        if (__any_sync(0xffffffffu, *abort_flag)) return;
+      }
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+        const float inv = 1.f / l[r];
+        T* out = static_cast<T*>(p.out) + (first + row[r]) * p.out_token +
+                 __shfl_sync(0xffffffffu, my_head, tq * 8 + r * 4) * p.out_head + c0 +
+                 (g >> 1) * 8 + (g & 1);
+#pragma unroll
+        for (int i = 0; i < 4 * NC; ++i)
+          out[(i / 4) * 32 + (i % 4) * 2] = static_cast<T>(acc[i / 2][(i & 1) * 2 + r] * inv);
+      }
+    }
+  }
 }
 
 template <typename T, int DQK, int DV>
@@ -931,17 +1061,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             __syncwarp();
           }
         }
-        uint32_t again = __ballot_sync(0xffffffffu, live && !(odd.x + odd.y == 0.f));
+        // A sum that is not finite is that of the row's own scores: NaN it stays.
+        const uint32_t again =
+            __ballot_sync(0xffffffffu, live && !(odd.x + odd.y == 0.f) && isfinite(inv));
         if (again) {  // these rows are written once more, after the stores above
           if (lane == 0) bulk_wait_group_all();
           __syncwarp();
-        }
-        for (; again; again &= again - 1) {
-          const int src = __ffs(again) - 1;
-          // Keys that the row's MMAs covered, up to a whole step past its tile.
+          // Keys that the rows' MMAs covered, up to a whole step past their tile.
           const int32_t covered = min(item.len, (end_of(item, s) + 15) / 16 * 16);
-          exact_row<T, DQK, DV>(p, item.first, __shfl_sync(0xffffffffu, tok, src), item.kvh,
-                                __shfl_sync(0xffffffffu, head, src), covered);
+          redo_rows<T, DQK, DV>(p, again, item.first, tok0, tok, item.kvh, head, covered,
+                                abort_flag);
         }
       }
     }
@@ -1183,7 +1312,10 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
   // scores, -inf, to -inf: any factor far below the scores' rounding will do.
   p.qscale = fabsf(g.scale) * 1.4426950408889634f;
   if (!(p.qscale >= 1e-30f)) p.qscale = 1e-30f;
-  p.timeout_ns = wait_timeout_ns();
+  // The output warps may redo 64 rows (redo_rows) between two reads of TMEM, for
+  // which the others wait: 20 ns a row and key with heads of 128, 90 with 64 heads of
+  // 192 / 128 out of DRAM.  1000 are allowed beyond the usual limit.
+  p.timeout_ns = wait_timeout_ns() + static_cast<uint64_t>(p.max_seqlen) * 64 * 1000;
   // No more items than the whole blocks of all tokens and one ragged one a
   // sequence, nor than every sequence at its longest.
   const int64_t per = 2 * tq;

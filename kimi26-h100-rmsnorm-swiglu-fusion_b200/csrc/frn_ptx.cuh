@@ -520,6 +520,26 @@ __device__ __forceinline__ uint32_t float2_to_pair<__half>(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&r);
 }
 
+// c += a . b on one warp (16 rows, 8 columns, 16 terms).
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (sizeof(T) == 2) {
+    if constexpr (Elem16<T>::kUmmaFormat == 1u)
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
 // Epilogue staging for a TMA tensor store.  Lane r holds row r of a warp's
 // 32-row block as fp32 accumulator columns v[0 .. 8*NJ); each value is
 // multiplied by `scale` (the row's inv_rms) and, with COLSCALE, by the

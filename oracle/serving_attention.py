@@ -33,6 +33,17 @@ def assert_close(got: torch.Tensor, ref: torch.Tensor, spread: torch.Tensor) -> 
     assert worst <= 0.0, f"off by {worst:.3g} more than the bound"
 
 
+def assert_same(got: torch.Tensor, ref: torch.Tensor, spread: torch.Tensor) -> None:
+    """assert_close, and infinite exactly where ref is, by sign."""
+    infinite = torch.isinf(ref)
+    g = got.double().cpu()
+    assert torch.equal(g[infinite], ref[infinite]), "other infinities than the oracle's"
+    assert not torch.isinf(g[~infinite]).any(), "infinities in other places than the oracle's"
+    finite = torch.isfinite(ref)
+    assert torch.equal(torch.isnan(g), torch.isnan(ref)), "NaN in other places than the oracle's"
+    assert_close(got[finite.to(got.device)], ref[finite], spread[finite])
+
+
 def _attend(q, k, v, scale, causal):
     """q [n, Hq, D] against k, v [m, Hkv, *] -> (out, spread) [n, Hq, Dv]."""
     group = q.shape[1] // k.shape[1]
