@@ -465,9 +465,12 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
         }
         // fp16: P is kept 2^15 higher, so that fewer small ones fall below the
         // type's normal range; sums and parts carry the same factor.
-        const float shift = Elem16<T>::kUmmaFormat == 0u ? 15.f - m_new : -m_new;
+        // The difference comes first, so that the largest P is 2^15 whatever the
+        // size of the scores: 15 - m alone would be rounded, by more than one from
+        // 2^24 on, and P leave the type's range.
+        constexpr float kUp = Elem16<T>::kUmmaFormat == 0u ? 15.f : 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = exp2_approx(x[e] + shift);
+        for (int e = 0; e < 4; ++e) x[e] = exp2_approx((x[e] - m_new) + kUp);
         l_run[r] += (x[0] + x[1]) + (x[2] + x[3]);
         pa[r] = float2_to_pair<T>(x[0], x[1]);
         pa[2 + r] = float2_to_pair<T>(x[2], x[3]);
