@@ -82,7 +82,11 @@ struct PagedDecodeParams {
   int32_t batch, hkv, group, warps;
   int32_t least, least_share;  // tiles that an item counts as, and that a share has, at least
   int32_t join_rows;  // query heads of a CTA of the join: 1 or 4
-  float qscale;    // scale * log2(e): the softmax runs in base 2
+  // scale * log2(e): the softmax runs in base 2.  16-bit: maxima (the parts' too) are
+  // those of the scaled scores, unit is 1.  fp32: of the unscaled ones, of a negated
+  // query where the scale is negative; qscale and unit are |scale| * log2(e).
+  float qscale, unit;
+  float qsign;
 };
 
 template <typename T, int D, int GMAX>
@@ -410,7 +414,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
         for (int r = 0; r < GMAX; ++r)
 #pragma unroll
           for (int e = 0; e < E; ++e)
-            qv[r][e] = r < G ? static_cast<float>(qp[r * p.q_head + e * 32 + lane]) : 0.f;
+            qv[r][e] =
+                r < G ? static_cast<float>(qp[r * p.q_head + e * 32 + lane]) * p.qsign : 0.f;
 #pragma unroll
         for (int r = 0; r < GMAX; ++r)
 #pragma unroll
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
 #pragma unroll
         for (int r = 0; r < HB; ++r) x[r] += __shfl_xor_sync(0xffffffffu, x[r], 16);
 #pragma unroll
-        for (int r = 0; r < HB; ++r) bm[r] = live ? x[r] * p.qscale : -FLT_MAX;
+        for (int r = 0; r < HB; ++r) bm[r] = live ? x[r] : -FLT_MAX;
 #pragma unroll
         for (int w = 8; w > 0; w >>= 1)
 #pragma unroll
@@ -533,7 +538,9 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
 #pragma unroll
           for (int r = 0; r < HB; ++r) {
             const float m_new = fmaxf(m_run[r4 + r], bm[r]);
-            const float corr = exp2f(m_run[r4 + r] - m_new);
+            const float corr = m_run[r4 + r] == -FLT_MAX
+                                   ? 0.f
+                                   : exp2f((m_run[r4 + r] - m_new) * p.qscale);
             m_run[r4 + r] = m_new;
             l_run[r4 + r] *= corr;
 #pragma unroll
@@ -542,7 +549,10 @@ __global__ void __launch_bounds__(kPagedThreads, paged_ctas_per_sm(sizeof(T) == 
         }
 #pragma unroll
         for (int r = 0; r < HB; ++r) {
-          s[r4 + r] = live ? exp2f(fmaf(x[r], p.qscale, -m_run[r4 + r])) : 0.f;
+          // The difference is taken before it is scaled: that of large scores (2^24 and
+          // more) is exact, and zero for the largest, where a rounding of the scaled
+          // ones would be worth a power of two.
+          s[r4 + r] = live ? exp2f((x[r] - m_run[r4 + r]) * p.qscale) : 0.f;
           l_run[r4 + r] += half == 0 ? s[r4 + r] : 0.f;  // one of the two copies counts
         }
       }
@@ -679,7 +689,8 @@ __device__ __forceinline__ void join_parts(const PagedDecodeParams& p, const flo
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const float m_new = fmaxf(mx, ml[i].x), c = exp2f(mx - m_new), f = exp2f(ml[i].x - m_new);
+      const float m_new = fmaxf(mx, ml[i].x);
+      const float c = exp2f((mx - m_new) * p.unit), f = exp2f((ml[i].x - m_new) * p.unit);
       mx = m_new;
       den = fmaf(ml[i].y, f, den * c);
 #pragma unroll
@@ -741,7 +752,7 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const PagedDecodePar
       float num = 0.f, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        const float f = exp2f(sm_ml[w].x - m);
+        const float f = exp2f((sm_ml[w].x - m) * p.unit);
         num = fmaf(sm_acc[w][d], f, num);
         sum = fmaf(sm_ml[w].y, f, sum);
       }
@@ -863,7 +874,13 @@ int run_paged_decode(const PagedDecodeProblem& g, cudaStream_t stream) {
   p.ws = static_cast<float*>(g.workspace);
   p.joins = reinterpret_cast<int32_t*>(
       p.ws + static_cast<int64_t>(2 * p.warps) * p.group * (g.kv.head_dim + 2));
-  p.qscale = g.scale * 1.4426950408889634f;  // log2(e): the softmax runs in base 2
+  p.qscale = g.scale * 1.4426950408889634f;  // log2(e)
+  p.unit = 1.f;
+  p.qsign = 1.f;
+  if (g.dtype == FRN_DTYPE_F32) {
+    p.qsign = g.scale < 0.f ? -1.f : 1.f;
+    p.unit = p.qscale = fabsf(p.qscale);
+  }
   switch (g.dtype) {
     case FRN_DTYPE_BF16: return launch_paged_d<__nv_bfloat16>(g, p, stream);
     case FRN_DTYPE_F16: return launch_paged_d<__half>(g, p, stream);

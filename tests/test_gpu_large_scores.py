@@ -34,7 +34,7 @@ def keys(n, Hkv, D, size, pattern, dtype):
 PATTERNS = ["equal", "negative", "blocks", "one"]
 
 
-@pytest.mark.parametrize("dtype,size", [(d, s) for d in (torch.float16,) for s in SIZES[d]],
+@pytest.mark.parametrize("dtype,size", [(d, s) for d in SIZES for s in SIZES[d]],
                          ids=lambda x: IDS.get(x, str(x)))
 @pytest.mark.parametrize("pattern", PATTERNS)
 @pytest.mark.parametrize("D", [64, 128])
