@@ -77,7 +77,8 @@ constexpr int kOut = 8, kLoadQK = 12, kMma = 13, kLoadV = 15;
 constexpr int kAhead = 6;      // K/V tiles before its end that an item's successor is found
 constexpr int kItemSlots = 4;  // items that the scheduler is ahead
 constexpr float kLag = 8.f;    // log2 of the most that a probability may exceed 1
-constexpr float kFloor = -1e30f;  // least first maximum: scores of -inf alone are not one
+constexpr float kFar = 0x1p14f;   // scaled scores from which on differences are taken first
+constexpr float kFloor = -FLT_MAX;  // least first maximum: scores of -inf alone are not one
 
 // Two row tiles of one KV head: tokens from t0 on of the sequence in rows
 // [first, first + len).  len = 0: no more items.
@@ -1177,18 +1178,33 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         float m_tile = max_of(0, kFloor);
         if (j == 0) m_used = m_tile;
         uint32_t w[16];
+        float less = 0.f;  // what was taken from the scores beforehand
 #pragma unroll 1
         for (;;) {
           piece(x, w);
 #pragma unroll
           for (int h = 1; h < kKeys / 32; ++h) m_tile = max_of(h, m_tile);
-          const bool grow = (m_tile - m_used) * p.qscale > kLag;
-          if (!__any_sync(0xffffffffu, grow)) break;
+          // -m * scale is rounded, which moves a row's exponents.  Beyond kFar that
+          // would tell in the weights, and from 2^24 on be a power of two or more:
+          // there the difference is taken first, once the maximum is known.
+          // A row is in order after one time through the rest: its maximum is then at
+          // most kLag behind, and near zero.
+          const auto is_far = [](float m) { return fabsf(m) * (kLag / kFar); };
+          const float rise = m_tile - m_used;
+          if (!__any_sync(0xffffffffu, fmaxf(rise, is_far(m_used)) * p.qscale > kLag)) break;
+          const bool grow = rise * p.qscale > kLag;
           const float m_new = grow ? m_tile : m_used;
-          if (j > 0)
+          if (j > 0 && __any_sync(0xffffffffu, grow))
             move_max(m_new);
           else
             m_used = m_new;
+          if (is_far(m_used) * p.qscale > kLag) {
+            less = m_used;
+            m_tile -= less;
+            m_used = 0.f;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) x[i] -= less;
+          }
           sum = make_float2(0.f, 0.f);
         }
         store(0, w);
@@ -1206,6 +1222,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           store(h, w);
         }
         l += sum.x + sum.y;
+        m_used += less;
       }
       // The sums go to the output warps, by two slots (and barriers) in turn: the
       // first product of the next item waits for the output of this one, so the

@@ -56,3 +56,35 @@ def decode(dtype, size, pattern, D):
     assert torch.isfinite(got).all()
     orc.assert_same(got, ref, spread)
     assert capi.device_error(0) == 0
+
+
+@pytest.mark.parametrize("dtype,size", [(d, s) for d in SIZES if d != torch.float32
+                                        for s in SIZES[d]], ids=lambda x: IDS.get(x, str(x)))
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("dims", [(4, 2, 128, 128), (7, 1, 64, 64), (2, 2, 192, 128)],
+                         ids=lambda x: "x".join(map(str, x)))
+def test_prompt(dtype, size, pattern, dims):
+    prompt(dtype, size, pattern, dims)
+
+
+def prompt(dtype, size, pattern, dims):
+    Hq, Hkv, Dqk, Dv = dims
+    lens = [300, 1, 45]
+    cu = [0, 300, 301, 346]
+    q = torch.full((346, Hq, Dqk), size).to(dtype)
+    k = torch.cat([keys(n, Hkv, Dqk, size, pattern, dtype) for n in lens])
+    v = torch.randn(346, Hkv, Dv, generator=torch.Generator().manual_seed(2)).to(dtype)
+    got = capi.gqa_prompt_attention(q.to(DEV), k.to(DEV), v.to(DEV),
+                                    torch.tensor(cu, dtype=torch.int32, device=DEV), 300,
+                                    Dqk ** -0.5)
+    ref, spread = orc.prompt_attention(q, k, v, cu, Dqk ** -0.5)
+    assert torch.isfinite(got).all()
+    orc.assert_same(got, ref, spread)
+    assert capi.device_error(0) == 0
+
+
+@pytest.mark.parametrize("dims", [(4, 2, 128, 128), (7, 1, 64, 64), (2, 2, 192, 128)],
+                         ids=lambda x: "x".join(map(str, x)))
+def test_prompt_of_very_low_scores(dims):
+    """Every score far below -1e30."""
+    prompt(torch.bfloat16, 2.0 ** 55, "negative", dims)
