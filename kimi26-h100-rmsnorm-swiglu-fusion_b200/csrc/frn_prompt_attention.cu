@@ -1328,7 +1328,7 @@ static int launch_prompt(const PromptProblem& g, cudaStream_t stream) {
   // A scale of zero (every key the same weight) still has to send the masked
   // scores, -inf, to -inf: any factor far below the scores' rounding will do.
   p.qscale = fabsf(g.scale) * 1.4426950408889634f;
-  if (!(p.qscale >= 1e-30f)) p.qscale = 1e-30f;
+  if (p.qscale < 1e-30f) p.qscale = 1e-30f;  // a NaN stays
   // The output warps may redo 64 rows (redo_rows) between two reads of TMEM, for
   // which the others wait: 20 ns a row and key with heads of 128, 90 with 64 heads of
   // 192 / 128 out of DRAM.  1000 are allowed beyond the usual limit.
