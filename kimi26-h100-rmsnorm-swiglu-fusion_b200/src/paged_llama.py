@@ -72,11 +72,11 @@ class PagedLlama:
         seqs = [self.cache.new_sequence() for _ in prompts]
         try:
             step = self.cache.extend(seqs, [len(p) for p in prompts])
+            return seqs, self._forward(step, [t for p in prompts for t in p], True)
         except Exception:
             for s in seqs:
                 self.cache.free(s)
             raise
-        return seqs, self._forward(step, [t for p in prompts for t in p], True)
 
     def decode(self, seqs: list[int], tokens: list[int]) -> torch.Tensor:
         """One more token of each sequence; logits [batch, vocab]."""
@@ -85,15 +85,17 @@ class PagedLlama:
         return self._forward(self.cache.extend(seqs, [1] * len(seqs)), tokens, False)
 
     def generate(self, prompts: list[list[int]], max_new_tokens: int) -> list[list[int]]:
-        """Greedy continuations; the sequences are freed afterwards."""
+        """Greedy continuations; the sequences are freed afterwards, also where a step fails."""
         seqs, logits = self.prefill(prompts)
         out: list[list[int]] = [[] for _ in prompts]
-        for n in range(max_new_tokens):
-            tokens = logits.argmax(-1).tolist()
-            for o, t in zip(out, tokens):
-                o.append(t)
-            if n + 1 < max_new_tokens:
-                logits = self.decode(seqs, tokens)
-        for s in seqs:
-            self.cache.free(s)
+        try:
+            for n in range(max_new_tokens):
+                tokens = logits.argmax(-1).tolist()
+                for o, t in zip(out, tokens):
+                    o.append(t)
+                if n + 1 < max_new_tokens:
+                    logits = self.decode(seqs, tokens)
+        finally:
+            for s in seqs:
+                self.cache.free(s)
         return out

@@ -1,0 +1,59 @@
+"""The serving loop when a step fails, without a GPU: the model's forward is a stand-in, the cache
+the host bookkeeping alone.  What a failed call took is given back."""
+import pytest
+import torch
+
+from src.paged_kv_cache import OutOfPages, PageAllocator
+from src.paged_llama import PagedLlama
+
+
+class Broken(RuntimeError):
+    pass
+
+
+class Cache(PageAllocator):
+    def extend(self, seqs, counts):
+        super().extend(seqs, counts)
+        return len(seqs)
+
+
+def make(num_pages, page_size, fails=()):
+    """A server whose forward raises at the calls numbered in `fails`."""
+    server = PagedLlama.__new__(PagedLlama)
+    server.cache = Cache(num_pages, page_size)
+    server.calls = 0
+
+    def forward(step, tokens, prompt):
+        server.calls += 1
+        if server.calls in fails:
+            raise Broken("forward")
+        return torch.zeros(step, 10)
+
+    server._forward = forward
+    return server
+
+
+def test_generate_gives_its_pages_back():
+    server = make(4, 4)
+    kept = server.cache.new_sequence()
+    with pytest.raises(OutOfPages):
+        server.generate([[1] * 6, [2] * 6], 8)  # two pages each, and a third for the ninth token
+    assert server.cache.free_pages == 4 and server.cache.sequences() == [kept]
+    assert server.generate([[1] * 6], 3) == [[0, 0, 0]]
+    assert server.cache.free_pages == 4 and server.cache.sequences() == [kept]
+
+
+@pytest.mark.parametrize("call", [1, 2, 3])
+def test_a_failing_forward_gives_its_pages_back(call):
+    server = make(8, 4, fails=(call,))
+    with pytest.raises(Broken):
+        server.generate([[1] * 6, [2] * 3], 4)
+    assert server.cache.free_pages == 8 and server.cache.sequences() == []
+
+
+def test_a_failing_prefill_leaves_the_others():
+    server = make(8, 4, fails=(2,))
+    seqs, _ = server.prefill([[1, 2, 3]])
+    with pytest.raises(Broken):
+        server.prefill([[4] * 9, [5]])
+    assert server.cache.sequences() == seqs and server.cache.free_pages == 7
