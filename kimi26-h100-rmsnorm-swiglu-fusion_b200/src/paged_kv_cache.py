@@ -141,6 +141,19 @@ class PageAllocator:
             self._length[seq] = length + n
         return moves
 
+    def withdraw(self, seqs: list[int], counts: list[int]) -> None:
+        """Takes the last counts[i] tokens of seqs[i] back: those of a step that failed."""
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
+            raise ValueError("withdraw: one count for each of different sequences")
+        for seq, n in zip(seqs, counts):
+            if not 0 <= n <= self._length[self._known(seq)]:
+                raise ValueError(f"withdraw: {n} tokens of a sequence of {self._length[seq]}")
+        for seq, n in zip(seqs, counts):
+            self._length[seq] -= n
+            pages = self._pages[seq]
+            while (len(pages) - 1) * self.page_size >= self._length[seq] and pages:
+                self._drop(pages.pop())
+
     def compact(self) -> list[tuple[int, int]]:
         """Renumbers the live pages to 0 .. n - 1; the pages to move."""
         live = sum(u > 0 for u in self._uses)

@@ -79,10 +79,16 @@ class PagedLlama:
             raise
 
     def decode(self, seqs: list[int], tokens: list[int]) -> torch.Tensor:
-        """One more token of each sequence; logits [batch, vocab]."""
+        """One more token of each sequence; logits [batch, vocab].  Where this fails the
+        sequences are as before, and the call can be made again."""
         if len(tokens) != len(seqs):
             raise ValueError("decode: one token a sequence")
-        return self._forward(self.cache.extend(seqs, [1] * len(seqs)), tokens, False)
+        step = self.cache.extend(seqs, [1] * len(seqs))
+        try:
+            return self._forward(step, tokens, False)
+        except Exception:
+            self.cache.withdraw(seqs, [1] * len(seqs))
+            raise
 
     def generate(self, prompts: list[list[int]], max_new_tokens: int) -> list[list[int]]:
         """Greedy continuations; the sequences are freed afterwards, also where a step fails."""

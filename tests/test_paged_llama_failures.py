@@ -57,3 +57,41 @@ def test_a_failing_prefill_leaves_the_others():
     with pytest.raises(Broken):
         server.prefill([[4] * 9, [5]])
     assert server.cache.sequences() == seqs and server.cache.free_pages == 7
+
+
+def test_a_failing_decode_can_be_repeated():
+    server = make(8, 4, fails=(2,))
+    seqs, _ = server.prefill([[1] * 4, [2] * 3])
+    fork = server.cache.fork(seqs[1])
+    before = [server.cache.length(s) for s in seqs + [fork]], server.cache.free_pages
+    with pytest.raises(Broken):
+        server.decode(seqs, [5, 6])
+    assert [server.cache.length(s) for s in seqs + [fork]] == before[0]
+    # The page that seqs[1] shared has been copied for it; a page of no token is not kept.
+    assert server.cache.free_pages == before[1] - 1
+    assert server.decode(seqs, [5, 6]).shape == (2, 10)
+    assert [server.cache.length(s) for s in seqs + [fork]] == [5, 4, 3]
+    for s in seqs + [fork]:
+        server.cache.free(s)
+    assert server.cache.free_pages == 8
+
+
+def test_withdraw():
+    a = PageAllocator(10, 4)
+    s, t = a.new_sequence(), a.new_sequence()
+    a.extend([s, t], [9, 4])
+    for n, pages in ((0, 3), (1, 2), (3, 2), (1, 1), (4, 0)):
+        a.withdraw([s], [n])
+        assert len(a.pages(s)) == pages == -(-a.length(s) // 4)
+    assert a.length(s) == 0 and a.free_pages == 9
+    a.extend([s], [5])
+    f = a.fork(s)
+    a.withdraw([s, t], [5, 0])
+    assert a.length(f) == 5 and len(a.pages(f)) == 2 and a.free_pages == 7
+    with pytest.raises(ValueError, match="5 tokens of a sequence of 4"):
+        a.withdraw([f, t], [1, 5])
+    with pytest.raises(ValueError, match="one count"):
+        a.withdraw([t, t], [1, 1])
+    with pytest.raises(KeyError, match="no sequence"):
+        a.withdraw([99], [1])
+    assert a.length(f) == 5 and a.length(t) == 4
