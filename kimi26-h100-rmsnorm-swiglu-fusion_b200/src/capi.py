@@ -391,16 +391,36 @@ def gqa_decode_attention_noalloc(q, k_cache, v_cache, scale: float, out):
     return out
 
 
+def _check_heads(like, **tensors) -> None:
+    """3-D tensors [tokens, heads, dim] of like's dtype and device, unit stride along dim."""
+    for name, t in tensors.items():
+        assert t.dim() == 3 and t.dtype == like.dtype and t.device == like.device, name
+        assert t.stride(2) == 1 or t.shape[2] == 1 or t.numel() == 0, name
+
+
+def _check_ints(like, **tensors) -> None:
+    """int32 tensors on like's device, unit stride along the last dim."""
+    for name, t in tensors.items():
+        assert str(t.dtype) == "torch.int32" and t.device == like.device, name
+        assert t.stride(-1) == 1 or t.shape[-1] <= 1 or t.numel() == 0, name
+
+
 def gqa_prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out=None):
     """Causal attention over packed prompts through the C ABI: q [T, Hq, Dqk],
     k [T, Hkv, Dqk], v [T, Hkv, Dv], cu_seqlens int32 [B + 1] on the GPU;
     returns out [T, Hq, Dv]."""
     import torch
 
+    _check_heads(q, q=q, k=k, v=v)
+    _check_ints(q, cu_seqlens=cu_seqlens)
     T, Hq, Dqk = q.shape
     Hkv, Dv = v.shape[1], v.shape[2]
+    assert tuple(k.shape) == (T, Hkv, Dqk) and v.shape[0] == T
+    assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1
     if out is None:
         out = torch.empty(T, Hq, Dv, dtype=q.dtype, device=q.device)
+    _check_heads(q, out=out)
+    assert tuple(out.shape) == (T, Hq, Dv)
     with _on(q.device):
         rc = lib().frn_gqa_prompt_attention(
             _dtype_code(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
@@ -413,6 +433,11 @@ def gqa_prompt_attention(q, k, v, cu_seqlens, max_seqlen: int, scale: float, out
 
 def paged_kv(k_pages, v_pages, page_table) -> PagedKV:
     """The struct frn_paged_kv of pools [P, page_size, Hkv, D] and a table [B, max_pages]."""
+    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape
+    assert k_pages.dtype == v_pages.dtype and k_pages.device == v_pages.device
+    assert (k_pages.stride(3) == 1 and v_pages.stride(3) == 1) or k_pages.numel() == 0
+    assert page_table.dim() == 2
+    _check_ints(k_pages, page_table=page_table)
     P, page_size, Hkv, D = k_pages.shape
     return PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), P, page_size, Hkv, D,
                    k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), v_pages.stride(0),
@@ -427,10 +452,16 @@ def gqa_paged_decode_attention(q, k_pages, v_pages, page_table, seq_lens, scale:
     and seq_lens int32 [B] on the GPU; returns out [B, Hq, D]."""
     import torch
 
+    _check_heads(q, q=q)
+    _check_ints(q, seq_lens=seq_lens)
     B, Hq, D = q.shape
     if out is None:
         out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    _check_heads(q, out=out)
+    assert out.shape == q.shape
     cache = paged_kv(k_pages, v_pages, page_table)
+    assert k_pages.dtype == q.dtype and k_pages.device == q.device and k_pages.shape[3] == D
+    assert tuple(seq_lens.shape) == (B,) and page_table.shape[0] == B
     with _on(q.device):
         if workspace is None:
             need = lib().frn_gqa_paged_decode_workspace_size(
@@ -446,7 +477,15 @@ def gqa_paged_decode_attention(q, k_pages, v_pages, page_table, seq_lens, scale:
 
 def kv_cache_append(k, v, k_pages, v_pages, page_table, start_lens, cu_seqlens=None) -> None:
     """Writes k, v [T, Hkv, D] to their sequences' pages through the C ABI."""
+    _check_heads(k, k=k, v=v)
+    _check_ints(k, start_lens=start_lens)
+    assert k.shape == v.shape and k.shape[1:] == k_pages.shape[2:]
     cache = paged_kv(k_pages, v_pages, page_table)
+    assert k_pages.dtype == k.dtype and k_pages.device == k.device
+    assert start_lens.dim() == 1 and page_table.shape[0] == start_lens.numel()
+    if cu_seqlens is not None:
+        _check_ints(k, cu_seqlens=cu_seqlens)
+        assert tuple(cu_seqlens.shape) == (start_lens.numel() + 1,)
     with _on(k.device):
         rc = lib().frn_kv_cache_append(
             _dtype_code(k), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
@@ -459,7 +498,13 @@ def kv_cache_append(k, v, k_pages, v_pages, page_table, start_lens, cu_seqlens=N
 def kv_pages_copy(pools, src, dst) -> None:
     """Copies pages src[i] -> dst[i] in every pool [P, ...] through the C ABI."""
     n = len(src)
-    assert len(dst) == n and all(p.shape == pools[0].shape for p in pools)
+    assert len(dst) == n and all(p.shape == pools[0].shape and p.stride() == pools[0].stride()
+                                 and p.dtype == pools[0].dtype and p.device == pools[0].device
+                                 for p in pools)
+    if pools[0].shape[0]:  # a page is one block, its dims in any order
+        page = pools[0][0]
+        order = sorted(range(page.dim()), key=lambda i: (-page.stride(i), -page.shape[i]))
+        assert page.permute(order).is_contiguous()
     ptrs = (c_void_p * len(pools))(*[p.data_ptr() for p in pools])
     first = pools[0]
     es = first.element_size()
