@@ -18,9 +18,10 @@
 // (at most two parts a warp: an item can be cut at its share's start and at
 // its end), and a second, dependent launch joins the parts in share order.  No
 // atomics: the result does not depend on the order in which warps finish.
-// Shares are a warp's, not a CTA's: with four warps on every tile the join of
-// the warps at each item's end cost 2 us, and a batch of 64 sequences of 1 to
-// 8192 tokens took 76 us instead of 45.
+// Shares are a warp's, not a CTA's: with four warps on every tile the warps had to
+// be joined at each item's end, and a batch of 64 sequences of 1 to 8192 tokens took
+// 96.8 us instead of 91.7, one of 1000 16.1 instead of 14.1 (both without the later
+// steps).
 //
 // Streams.  A warp copies its tiles with 16-byte cp.async into its own ring,
 // several tiles ahead and across item borders: no block barrier and no page
@@ -29,8 +30,8 @@
 // unused slots or pages has no effect.
 //
 // What bounds it: HBM.  8 sequences of 100 to 131 thousand tokens (3.8 GB) take
-// 596 to 631 us, 6.0 to 6.4 TB/s or 92 to 98% of a plain copy's rate; 64 sequences
-// of 1 to 8192 tokens (352 MB) 67 to 70 us, about 10 of them the start of the
+// 596 to 635 us, 6.0 to 6.4 TB/s or 92 to 98% of a plain copy's rate; 64 sequences
+// of 1 to 8192 tokens (352 MB) 67 to 71 us, about 10 of them the start of the
 // streams and the join; one sequence of 1000 tokens 8.5 us, of which a one-token
 // call's chain of dependent loads and two launches is 5.7.  Two CTAs an SM with
 // three tiles in flight a warp: one CTA with seven is 6 to 20% slower, three with
@@ -44,10 +45,12 @@
 // rounding to that, and costs 2 to 4% of the time).  fp32: CUDA cores, one
 // token a lane for the scores, head dims across lanes for the output.  Four heads'
 // scores are taken together, so that their shuffles and exponentials overlap: 8
-// sequences of 8192 tokens, 32 / 8 heads of 128, take 132 us instead of 158, and
-// 125 (4.3 TB/s) with eight tokens of the second product unrolled instead of four;
-// four warps an SM leave the latencies of shared memory uncovered.  Eight heads
-// together are 15% slower there and 2% faster with eight heads of 64.
+// sequences of 8192 tokens, 32 / 8 heads of 128, took 132 us instead of 158, and
+// another twentieth less with eight tokens of the second product unrolled instead of
+// four.  They take 132 us (4.1 TB/s) with the scores' differences taken before they
+// are scaled, 130.5 on the same card without; with rings of 16 KB tiles an SM holds
+// four warps, which leave the latencies of shared memory uncovered.  Eight heads
+// together were 15% slower there and 2% faster with eight heads of 64.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -764,9 +767,10 @@ __global__ void __launch_bounds__(32 * W) paged_join_kernel(const PagedDecodePar
 // ------------------------------------------------------------------ host side
 
 // 16-bit: an item's queries and end cost about what four tiles do, a part what two
-// do (one sequence of 1000 tokens: 8.9 us with shares of two, 10.2 with four; 64
-// sequences of 1 to 8192: 48 us where an item counts as two at least, 45 with
-// four).  fp32: the scores of a tile take longer than either.
+// do (one sequence of 1000 tokens: 9.6 us with shares of two, 11.3 with four; 64
+// sequences of 1 to 8192: 69.8 us where an item counts as four at least, 74.2 with
+// two, 88.3 with one; back to back, 352 MB a call).  fp32: the scores of a tile take
+// longer than either.
 static int paged_least(int dtype) { return dtype == FRN_DTYPE_F32 ? 1 : 4; }
 static int paged_least_share(int dtype) { return dtype == FRN_DTYPE_F32 ? 1 : 2; }
 
@@ -839,8 +843,8 @@ static int launch_paged(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaS
 template <typename T, int D>
 static int launch_paged_g(const PagedDecodeProblem& g, PagedDecodeParams& p, cudaStream_t s) {
   // fp32: one or two heads, one after the other, where four together would be
-  // mostly padding (8 sequences of 8192 tokens, 8 heads of their own: 107 us,
-  // a tenth less).
+  // mostly padding (8 sequences of 8192 tokens, 8 heads of their own, 114 us: a
+  // tenth less when it was taken).
   if constexpr (sizeof(T) == 4)
     if (p.group <= 2) return launch_paged<T, D, 4>(g, p, s);
   return p.group <= 8 ? launch_paged<T, D, 8>(g, p, s) : launch_paged<T, D, 16>(g, p, s);

@@ -41,17 +41,26 @@
 // for the second product; the row sums are of the unrounded values, in fp32.
 //
 // What bounds it.  Of a K/V tile and both row tiles the tensor core has 2048
-// clocks of work (D = 128), the special-function units 2048; a round takes about
-// 2600: the way of one row tile from a finished S through its exponentials, the
-// rest of PV and the next S, and two barriers.  One prompt of 8192 tokens, 32 / 8
-// heads of 128, bf16: 401 to 417 us (1320 to 1370 TFLOP/s) in short runs at 1.73
-// GHz, 469 to 490 us (1120 to 1170 TFLOP/s) without pause, where the power limit
-// holds the clock at 1.49 GHz; MLA heads (192 / 128) of 500 to 2048 tokens 240 us
-// (790 TFLOP/s; 13% of the products are masked parts of diagonal tiles), 24 packed
-// prompts of 16 to 1500 tokens 97 to 99 us (680 TFLOP/s; items of one to twelve
-// tiles: the first tile's maximum cannot be guessed).  The instructions of a round
-// should stay in cache: one copy of the tile code for whole and masked tiles, 16 KB
-// less, took 500 us to 485.
+// clocks of work (D = 128), the special-function units 2048; a round takes 3000
+// (time x sampled clock over rounds an SM, 16384 to 65536 tokens): the way of one row
+// tile from a finished S through its exponentials, the rest of PV and the next S,
+// and two barriers.  One prompt of 8192 tokens, 32 / 8 heads of 128, bf16: 401 to 417
+// us (1320 to 1370 TFLOP/s) in short runs at 1.73 GHz, 466 to 480 us (1150 to 1180
+// TFLOP/s) without pause, where the power limit holds the clock at 1.5 GHz.  Short
+// prompts lose as much between items: 24 packed ones of 16 to 1500 tokens take 95 to
+// 98 us (680 to 700 TFLOP/s), 159 thousand clocks for 33 rounds and 8.5 items an SM,
+// so some 7000 an item beside its rounds; MLA heads (192 / 128, 2700 clocks a round of
+// 96 keys) of 500 to 2048 tokens 239 to 245 us (780 to 800 TFLOP/s), 366 thousand for
+// 105 rounds and 9.9 items, 8400 an item.  In these are the start, the uneven end
+// and the change of items; they were not told apart.  13% of the MLA products are
+// masked parts of diagonal tiles.  Finding an item reads all lengths again where there
+// are more than 32: 32, 64, 256 and 1024 prompts of 100 tokens, 32 / 8 heads, take 27,
+// 49, 310 and 3930 us.  Heads of 64: 28 / 4 heads, 4096 tokens 92 us, 16384 1220 us
+// (790 TFLOP/s; 3000 clocks a round again, with 1024 of work for the tensor core and
+// 2048 for the special-function units).
+// The instructions of a round should stay in cache: one copy of the tile code for
+// whole and masked tiles, 16 KB less, took 500 us to 485.  Nor is there a register to
+// spare: what all warps use is spilled when any of them needs more.
 // Not adopted: a quarter or half of the exponentials by polynomial (no gain once
 // the registers sufficed, 2.5% at D = 64), two threads a row (the maximum has to
 // be agreed on: 611 us), spinning instead of suspended waits (3% slower).
