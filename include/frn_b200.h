@@ -311,10 +311,10 @@ int frn_gqa_decode_attention_noalloc(int dtype, const void* q, const void* k_cac
  * FRN_DEVERR_BAD_LENGTH.  Rows of no sequence are left as they are.
  * Scores, softmax statistics and output sums are fp32; the probabilities are
  * rounded to `dtype` for the product with v (one that becomes zero makes a NaN of
- * an infinity in v).  What lies in k and v after position i has no effect on row i, NaN and infinities included (a NaN or an
- * infinity in v makes up to 255 rows a KV head before it slower: they are computed
- * again, and the limit on waits inside the kernel is longer by 64 us a token of
- * max_seqlen for their sake).
+ * an infinity in v).  What lies in k and v after position i has no effect on row
+ * i, NaN and infinities included (a NaN or an infinity in v makes up to 255 rows a
+ * KV head before it slower: they are computed again, and the limit on waits inside
+ * the kernel is longer by 64 us a token of max_seqlen for their sake).
  * Replaces the library call that the reference's patched attention makes for
  * prompts (reference src/patch_llama.py:147-161).
  */

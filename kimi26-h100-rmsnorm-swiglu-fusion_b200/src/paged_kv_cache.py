@@ -207,6 +207,13 @@ class PagedKVCache(PageAllocator):
         """Room for counts[i] more tokens of seqs[i], pages shared with other
         sequences copied where the step writes to them."""
         self._move(super().extend(seqs, counts))
+        try:
+            return self._step(seqs, counts)
+        except Exception:  # no memory for the step's arrays
+            self.withdraw(seqs, counts)
+            raise
+
+    def _step(self, seqs: list[int], counts: list[int]) -> Step:
         after = [self._length[s] for s in seqs]
         before = [a - n for a, n in zip(after, counts)]
         cu = [0]

@@ -3,7 +3,8 @@ the host bookkeeping alone.  What a failed call took is given back."""
 import pytest
 import torch
 
-from src.paged_kv_cache import OutOfPages, PageAllocator
+from src import paged_kv_cache
+from src.paged_kv_cache import OutOfPages, PageAllocator, PagedKVCache
 from src.paged_llama import PagedLlama
 
 
@@ -95,3 +96,21 @@ def test_withdraw():
     with pytest.raises(KeyError, match="no sequence"):
         a.withdraw([99], [1])
     assert a.length(f) == 5 and a.length(t) == 4
+
+
+def test_a_step_without_memory_is_taken_back(monkeypatch):
+    cache = PagedKVCache(1, 8, 4, 1, 64, device="cpu")
+    s = cache.new_sequence()
+    cache.extend([s], [3])
+
+    def no_memory(*args, **kwargs):
+        raise MemoryError("step")
+
+    with monkeypatch.context() as m:
+        m.setattr(paged_kv_cache.torch, "tensor", no_memory)
+        with pytest.raises(MemoryError):
+            cache.extend([s], [9])
+    assert cache.length(s) == 3 and cache.free_pages == 7
+    step = cache.extend([s], [9])
+    assert step.start_lens.tolist() == [3] and step.seq_lens.tolist() == [12]
+    assert step.positions.tolist() == list(range(3, 12)) and not step.fresh
